@@ -1,0 +1,257 @@
+// Bindings of the language-model operators: attention with shaped scores (attn_shaped.hip), token log
+// probabilities (logprobs.hip), token order and the embedding gradient summed in it (embed_sort.hip).
+// Every operand is checked (device, type, layout, extents, alignment) before a launch; launches go to
+// the current stream of the operands' device, workspaces come from the caching allocator of that stream
+// (so a captured graph owns the ones it uses).
+#include <torch/extension.h>
+#include <ATen/hip/HIPContext.h>
+#include <hip/hip_runtime.h>
+#include <vector>
+
+#include "bind_util.h"
+
+extern "C" {
+int tfk_shaped_fwd(const void*, const void*, const void*, void*, float*, int, const long long*, const long long*,
+                   const int*, const int*, const int*, const int*, const float*, float, float, int, float,
+                   unsigned long long, hipStream_t);
+int tfk_shaped_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*,
+                   void*, int, const long long*, const long long*, const long long*, const int*, const int*, const int*,
+                   const int*, const float*, float, float, int, float, unsigned long long, hipStream_t);
+int tfk_doc_spans(const int*, long long, int, int*, hipStream_t);
+int tfk_logprobs_kmax();
+long long tfk_logprobs_ws(long long, int, int, int);
+int tfk_logprobs_fwd(const void*, int, const int*, int, int, long long, int, int, float*, float*, float*, float*, float*,
+                     int*, void*, hipStream_t);
+int tfk_logprobs_bwd(const void*, int, const int*, int, int, long long, int, int, const float*, const float*,
+                     const int*, const float*, const float*, const float*, void*, long long, int, hipStream_t);
+long long tfk_token_order_scratch(long long);
+int tfk_token_order(const int*, int, int, int*, int*, int*, hipStream_t);
+long long tfk_emb_sorted_part(long long, int);
+int tfk_emb_sorted(const int*, const int*, int, int, int, const void*, int, long long, float*, float*, float, int,
+                   hipStream_t);
+}
+
+namespace {
+using Opt = c10::optional<torch::Tensor>;
+hipStream_t stream_of(const torch::Tensor& t) { return at::hip::getCurrentHIPStream(t.device().index()).stream(); }
+void same_device(const torch::Tensor& t, const torch::Tensor& ref, const char* n) {
+  TORCH_CHECK(t.device() == ref.device(), n, " is on ", t.device(), ", expected ", ref.device());
+}
+void need_opt(const Opt& t, at::ScalarType dt, long long n, const torch::Tensor& ref, const char* name) {
+  if (!t.has_value() || !t->defined()) return;
+  need(*t, dt, name);
+  same_device(*t, ref, name);
+  TORCH_CHECK(t->numel() == n, name, " has ", t->numel(), " elements, expected ", n);
+}
+void need_vec(const torch::Tensor& t, at::ScalarType dt, long long n, const torch::Tensor& ref, const char* name) {
+  need(t, dt, name);
+  same_device(t, ref, name);
+  TORCH_CHECK(t.numel() == n, name, " has ", t.numel(), " elements, expected ", n);
+}
+// 0 bf16, 1 f16, 2 f32
+int type_code(const torch::Tensor& t, bool f32, const char* n) {
+  TORCH_CHECK(t.is_cuda(), n, " must be a GPU tensor");
+  const auto d = t.scalar_type();
+  TORCH_CHECK(d == at::kBFloat16 || d == at::kHalf || (f32 && d == at::kFloat), n, " has dtype ", d,
+              f32 ? ", expected bfloat16, float16 or float32" : ", expected bfloat16 or float16");
+  return d == at::kBFloat16 ? 0 : d == at::kHalf ? 1 : 2;
+}
+
+// A column view of a token-major buffer: W elements at column `off` of tokens `rs` apart, batches `bs` apart.
+// `write`: no two tokens may share memory.
+void check_cols(const torch::Tensor& t, const torch::Tensor& ref, long long off, long long bs, long long rs, long long B,
+                long long S, long long W, bool write, const char* n) {
+  TORCH_CHECK(t.is_cuda(), n, " must be a GPU tensor");
+  same_device(t, ref, n);
+  TORCH_CHECK(t.scalar_type() == ref.scalar_type(), n, " has dtype ", t.scalar_type(), ", expected ", ref.scalar_type());
+  TORCH_CHECK(t.dim() >= 2 && (t.size(-1) == 1 || t.stride(-1) == 1), n, " needs unit stride along its last dim");
+  TORCH_CHECK(off >= 0 && off + W <= t.size(-1), n, ": columns ", off, "..", off + W, " outside a width of ", t.size(-1));
+  TORCH_CHECK(rs % 8 == 0 && bs % 8 == 0 && off % 8 == 0, n, ": strides/offset must be multiples of 8 elements");
+  TORCH_CHECK(rs >= W || S == 1, n, ": token stride ", rs, " < ", W);
+  const long long have = (long long)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
+  TORCH_CHECK(bs >= 0 && off + (B - 1) * bs + (S - 1) * rs + W <= have, n, " too small for its shape");
+  TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) + 2 * off) % 16 == 0, n, " must be 16-byte aligned");
+  if (write)
+    TORCH_CHECK(B == 1 || bs >= (S - 1) * rs + W || (bs >= W && rs >= (B - 1) * bs + W), n, ": tokens overlap");
+}
+void check_shape(const std::vector<int64_t>& s, const std::vector<int64_t>& st, double scale, double cap, double p_drop) {
+  TORCH_CHECK(s.size() == 6 && st.size() == 8, "attention shape [B,H,Hk,Sq,Sk,D], strides [q,k,v,o: batch, token]");
+  for (auto v : s) TORCH_CHECK(v >= 1 && v <= 0x7fffffff, "bad attention shape");
+  TORCH_CHECK(s[1] % s[2] == 0, "heads must be a multiple of key heads");
+  TORCH_CHECK(s[5] == 64 || s[5] == 128, "head dim must be 64 or 128, got ", s[5]);
+  // query rows padded to whole tiles; block counts and row indices are 32-bit
+  TORCH_CHECK((s[3] + 128) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x3fffffff, "sequence too long");
+  TORCH_CHECK(((s[3] + 128) / 32 * (s[1] / s[2]) + s[4] / 64 + 2) * s[0] * s[2] <= 0x7fffffff, "attention grid too large");
+  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "scale must be positive, got ", scale);
+  TORCH_CHECK(cap >= 0.0 && std::isfinite(cap), "softcap must be >= 0, got ", cap);
+  TORCH_CHECK(p_drop >= 0.0 && p_drop < 1.0, "p_drop");
+}
+struct Masks {
+  const int *kv_len, *q_start, *prefix, *docs;
+  const float* slopes;
+};
+Masks masks(const Opt& kv_len, const Opt& q_start, const Opt& prefix, const Opt& docs, const Opt& slopes,
+            const std::vector<int64_t>& s, const torch::Tensor& ref) {
+  need_opt(kv_len, at::kInt, s[0], ref, "kv_len");
+  need_opt(q_start, at::kInt, s[0], ref, "q_start");
+  need_opt(prefix, at::kInt, s[0], ref, "prefix_len");
+  need_opt(docs, at::kInt, 2 * s[0] * s[4], ref, "docs");
+  need_opt(slopes, at::kFloat, s[1], ref, "slopes");
+  if (docs.has_value() && docs->defined()) need_aligned(*docs, 8, "docs");
+  return Masks{opt_ptr<const int>(kv_len), opt_ptr<const int>(q_start), opt_ptr<const int>(prefix),
+               opt_ptr<const int>(docs), opt_ptr<const float>(slopes)};
+}
+
+void shaped_fwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch::Tensor v, int64_t vo, torch::Tensor out,
+                torch::Tensor lse, std::vector<int64_t> shape, std::vector<int64_t> strides, Opt kv_len, Opt q_start,
+                Opt prefix, Opt docs, Opt slopes, double scale, double cap, bool causal, double p_drop, int64_t seed) {
+  const int f16 = type_code(q, false, "q");
+  const c10::DeviceGuard guard(q.device());
+  check_shape(shape, strides, scale, cap, p_drop);
+  const long long B = shape[0], H = shape[1], Hk = shape[2], Sq = shape[3], Sk = shape[4], D = shape[5];
+  check_cols(q, q, qo, strides[0], strides[1], B, Sq, H * D, false, "q");
+  check_cols(k, q, ko, strides[2], strides[3], B, Sk, Hk * D, false, "k");
+  check_cols(v, q, vo, strides[4], strides[5], B, Sk, Hk * D, false, "v");
+  check_cols(out, q, 0, strides[6], strides[7], B, Sq, H * D, true, "out");
+  need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
+  const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
+  std::vector<long long> sh(shape.begin(), shape.end()), st(strides.begin(), strides.end());
+  auto at = [](torch::Tensor& t, int64_t o) { return (void*)((char*)t.data_ptr() + 2 * o); };
+  check_rc(tfk_shaped_fwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), lse.data_ptr<float>(), f16, sh.data(), st.data(),
+                          m.kv_len, m.q_start, m.prefix, m.docs, m.slopes, (float)scale, (float)cap, causal ? 1 : 0,
+                          (float)p_drop, (unsigned long long)seed, stream_of(q)),
+           "shaped_fwd");
+}
+
+void shaped_bwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch::Tensor v, int64_t vo, torch::Tensor out,
+                torch::Tensor dout, torch::Tensor lse, torch::Tensor dq, int64_t dqo, torch::Tensor dk, int64_t dko,
+                torch::Tensor dv, int64_t dvo, std::vector<int64_t> shape, std::vector<int64_t> strides,
+                std::vector<int64_t> gstrides, Opt kv_len, Opt q_start, Opt prefix, Opt docs, Opt slopes, double scale,
+                double cap, bool causal, double p_drop, int64_t seed) {
+  const int f16 = type_code(q, false, "q");
+  const c10::DeviceGuard guard(q.device());
+  check_shape(shape, strides, scale, cap, p_drop);
+  TORCH_CHECK(gstrides.size() == 6, "gstrides [dq,dk,dv: batch, token]");
+  const long long B = shape[0], H = shape[1], Hk = shape[2], Sq = shape[3], Sk = shape[4], D = shape[5];
+  check_cols(q, q, qo, strides[0], strides[1], B, Sq, H * D, false, "q");
+  check_cols(k, q, ko, strides[2], strides[3], B, Sk, Hk * D, false, "k");
+  check_cols(v, q, vo, strides[4], strides[5], B, Sk, Hk * D, false, "v");
+  check_cols(out, q, 0, strides[6], strides[7], B, Sq, H * D, false, "out");
+  check_cols(dout, q, 0, strides[6], strides[7], B, Sq, H * D, false, "dout");
+  check_cols(dq, q, dqo, gstrides[0], gstrides[1], B, Sq, H * D, true, "dq");
+  check_cols(dk, q, dko, gstrides[2], gstrides[3], B, Sk, Hk * D, true, "dk");
+  check_cols(dv, q, dvo, gstrides[4], gstrides[5], B, Sk, Hk * D, true, "dv");
+  need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
+  const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
+  torch::Tensor delta = torch::empty({B * H * Sq}, lse.options());
+  std::vector<long long> sh(shape.begin(), shape.end()), st(strides.begin(), strides.end()),
+      gs(gstrides.begin(), gstrides.end());
+  auto at = [](torch::Tensor& t, int64_t o) { return (void*)((char*)t.data_ptr() + 2 * o); };
+  check_rc(tfk_shaped_bwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
+                          delta.data_ptr<float>(), at(dq, dqo), at(dk, dko), at(dv, dvo), f16, sh.data(), st.data(),
+                          gs.data(), m.kv_len, m.q_start, m.prefix, m.docs, m.slopes, (float)scale, (float)cap,
+                          causal ? 1 : 0, (float)p_drop, (unsigned long long)seed, stream_of(q)),
+           "shaped_bwd");
+}
+
+void doc_spans(torch::Tensor ids, torch::Tensor out) {
+  need(ids, at::kInt, "ids");
+  TORCH_CHECK(ids.dim() == 2 && ids.size(1) <= 0x3fffffff, "ids must be [B, S]");
+  need_vec(out, at::kInt, 2 * ids.numel(), ids, "out");
+  need_aligned(out, 8, "out");
+  const c10::DeviceGuard guard(ids.device());
+  check_rc(tfk_doc_spans(ids.data_ptr<int>(), ids.size(0), (int)ids.size(1), out.data_ptr<int>(), stream_of(ids)),
+           "doc_spans");
+}
+
+// logits [T, cols] (unit column stride), the first V columns are classes
+int check_logits(const torch::Tensor& x, const torch::Tensor& ids, int64_t V, int64_t k) {
+  const int dt = type_code(x, true, "logits");
+  TORCH_CHECK(x.dim() == 2 && (x.size(1) == 1 || x.stride(1) == 1), "logits must be [T, V] with unit column stride");
+  TORCH_CHECK(V >= 1 && V <= x.size(1) && x.size(1) <= 0x3fffffff, "logits: ", V, " classes of ", x.size(1), " columns");
+  TORCH_CHECK(k >= 0 && k <= tfk_logprobs_kmax() && k <= V, "top_k must be in 0..min(", tfk_logprobs_kmax(), ", V), got ", k);
+  // blocks of a launch: rows times the parts of a row
+  TORCH_CHECK(x.size(0) * ((x.size(1) >> 12) + 1) <= 0x7fffffff, "too many rows");
+  need_vec(ids, at::kInt, x.size(0), x, "ids");
+  return dt;
+}
+void logprobs_fwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_t k, int64_t ignore, torch::Tensor logp,
+                  torch::Tensor ent, torch::Tensor lse, torch::Tensor norm, Opt top_logp, Opt top_ids) {
+  const int dt = check_logits(x, ids, V, k);
+  const c10::DeviceGuard guard(x.device());
+  const long long T = x.size(0);
+  need_vec(logp, at::kFloat, T, x, "logp"); need_vec(ent, at::kFloat, T, x, "entropy"); need_vec(lse, at::kFloat, T, x, "lse");
+  need_vec(norm, at::kFloat, 2 * T, x, "norm");
+  TORCH_CHECK(k == 0 || (top_logp.has_value() && top_ids.has_value()), "top_k needs its outputs");
+  need_opt(top_logp, at::kFloat, T * k, x, "top_logp");
+  need_opt(top_ids, at::kInt, T * k, x, "top_ids");
+  const long long ws = tfk_logprobs_ws(T, (int)V, dt, (int)k);
+  torch::Tensor w = torch::empty({ws}, x.options().dtype(at::kByte));
+  check_rc(tfk_logprobs_fwd(x.data_ptr(), dt, ids.data_ptr<int>(), (int)T, (int)V, x.stride(0), (int)k, (int)ignore,
+                            logp.data_ptr<float>(), ent.data_ptr<float>(), lse.data_ptr<float>(), norm.data_ptr<float>(),
+                            opt_ptr<float>(top_logp), opt_ptr<int>(top_ids), w.data_ptr(), stream_of(x)),
+           "logprobs_fwd");
+}
+void logprobs_bwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_t ignore, torch::Tensor norm, torch::Tensor ent,
+                  Opt top_ids, Opt dlogp, Opt dent, Opt dtop, torch::Tensor dx) {
+  const bool top = dtop.has_value() && dtop->defined();
+  TORCH_CHECK(!top || (top_ids.has_value() && top_ids->defined() && dtop->dim() == 2), "dtop [T, k] needs top_ids");
+  const int64_t k = top ? dtop->size(1) : 0;
+  const int dt = check_logits(x, ids, V, k);
+  const c10::DeviceGuard guard(x.device());
+  const long long T = x.size(0);
+  need_vec(norm, at::kFloat, 2 * T, x, "norm"); need_vec(ent, at::kFloat, T, x, "entropy");
+  need_opt(dlogp, at::kFloat, T, x, "dlogp"); need_opt(dent, at::kFloat, T, x, "dentropy");
+  if (top) { need_opt(dtop, at::kFloat, T * k, x, "dtop"); need_opt(top_ids, at::kInt, T * k, x, "top_ids"); }
+  need_vec(dx, x.scalar_type(), T * x.size(1), x, "dlogits");
+  check_rc(tfk_logprobs_bwd(x.data_ptr(), dt, ids.data_ptr<int>(), (int)T, (int)V, x.stride(0), (int)k, (int)ignore,
+                            norm.data_ptr<float>(), ent.data_ptr<float>(), top ? opt_ptr<const int>(top_ids) : nullptr,
+                            opt_ptr<const float>(dlogp), opt_ptr<const float>(dent), top ? opt_ptr<const float>(dtop) : nullptr,
+                            dx.data_ptr(), x.size(1), (int)x.size(1), stream_of(x)),
+           "logprobs_bwd");
+}
+
+void token_order(torch::Tensor ids, int64_t V, torch::Tensor perm, torch::Tensor keys) {
+  need(ids, at::kInt, "ids");
+  const long long T = ids.numel();
+  TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 0x3fffffff, "token_order: V ", V, ", tokens ", T);
+  need_vec(perm, at::kInt, T, ids, "perm"); need_vec(keys, at::kInt, T, ids, "keys");
+  const c10::DeviceGuard guard(ids.device());
+  torch::Tensor w = torch::empty({tfk_token_order_scratch(T)}, ids.options());
+  check_rc(tfk_token_order(ids.data_ptr<int>(), (int)T, (int)V, perm.data_ptr<int>(), keys.data_ptr<int>(),
+                           w.data_ptr<int>(), stream_of(ids)),
+           "token_order");
+}
+void embedding_bwd_sorted(torch::Tensor perm, torch::Tensor keys, torch::Tensor dy, torch::Tensor dword, double scale,
+                          bool accumulate) {
+  const int dt = type_code(dy, true, "dy");
+  need(dword, at::kFloat, "dword");
+  same_device(dword, dy, "dword");
+  TORCH_CHECK(dy.dim() == 2 && dword.dim() == 2 && dy.size(1) == dword.size(1), "dy [T, W] and dword [V, W]");
+  const long long T = dy.size(0), V = dword.size(0), W = dy.size(1);
+  TORCH_CHECK(W >= 8 && W % 8 == 0 && W <= (1 << 20), "embedding width %8, got ", W);
+  TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 0x3fffffff, "embedding_bwd_sorted: V ", V, ", tokens ", T);
+  // blocks of a launch: a group of >= 8 lanes per 32 tokens and 64 columns, and one per 64 rows
+  TORCH_CHECK((T / 32 + 1) * (W / 64 + 1) / 4 + V / 64 + 2 <= 0x7fffffff, "embedding_bwd_sorted: grid too large");
+  TORCH_CHECK((dy.size(1) == 1 || dy.stride(1) == 1) && (T <= 1 || (dy.stride(0) >= W && dy.stride(0) % 8 == 0)),
+              "dy rows: unit column stride, row stride a multiple of 8");
+  need_aligned(dy, 16, "dy"); need_aligned(dword, 16, "dword");
+  need_vec(perm, at::kInt, T, dy, "order"); need_vec(keys, at::kInt, T, dy, "order");
+  const c10::DeviceGuard guard(dy.device());
+  torch::Tensor part = torch::empty({tfk_emb_sorted_part(T, (int)W)}, dword.options());
+  check_rc(tfk_emb_sorted(keys.data_ptr<int>(), perm.data_ptr<int>(), (int)T, (int)V, (int)W, dy.data_ptr(), dt,
+                          dy.stride(0), dword.data_ptr<float>(), part.data_ptr<float>(), (float)scale, accumulate ? 1 : 0,
+                          stream_of(dy)),
+           "embedding_bwd_sorted");
+}
+}  // namespace
+
+void register_lm_ops(pybind11::module& m) {
+  m.def("shaped_fwd", &shaped_fwd);
+  m.def("shaped_bwd", &shaped_bwd);
+  m.def("doc_spans", &doc_spans);
+  m.def("logprobs_fwd", &logprobs_fwd);
+  m.def("logprobs_bwd", &logprobs_bwd);
+  m.def("token_order", &token_order);
+  m.def("embedding_bwd_sorted", &embedding_bwd_sorted);
+}

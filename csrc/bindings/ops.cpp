@@ -955,6 +955,7 @@ void add(torch::Tensor a, torch::Tensor b, torch::Tensor y, double alpha, double
 }  // namespace
 
 void register_transformer_ops(pybind11::module& m);
+void register_lm_ops(pybind11::module& m);
 void register_ckpt_ops(pybind11::module& m);
 void register_comm_ops(pybind11::module& m);
 
@@ -1029,6 +1030,7 @@ PYBIND11_MODULE(_C, m) {
   m.def("gather_rows", &gather_rows);
   m.def("scatter_add_rows", &scatter_add_rows);
   register_transformer_ops(m);
+  register_lm_ops(m);
   register_ckpt_ops(m);
   register_comm_ops(m);
 }

@@ -1,0 +1,316 @@
+// hipcc-flags: -Xclang -target-feature -Xclang -packed-fp32-ops
+// Log probabilities of given tokens, with the entropy of each row's distribution and its k most
+// probable tokens, and their gradient, for gfx950.
+//
+// For a row x of V logits: lse = m + ln S, S = sum e^(x - m), m = max x;
+//   logp = (x[id] - m) - ln S,   entropy = lse - sum p x = ln S - Y / S with Y = sum (x - m) e^(x - m).
+// m and ln S are kept apart for the backward (norm): lse alone loses ln S where |m| is large (a row whose
+// logits all are a mask value).
+// Gradient of the row, with the incoming gl (logp), gh (entropy) and gt[j] (the alternatives):
+//   dx[v] = gl [v == id] + sum_j gt[j] [v == top[j]] - p (gl + sum_j gt[j] + gh (ln p + entropy)).
+//
+// Both directions read each logit once (memory bound). The forward cuts a row into parts of at most
+// NT * NV 16-byte vectors; a part lives in the registers of one block, which reduces it to (m, S, Y) and
+// its k best, and a second launch joins the parts of a row (a row of one part is finished at once).
+// So a few long rows fill the card as many short ones do. f32 sums throughout.
+#include "common.h"
+
+namespace {
+typedef _Float16 f16;
+typedef unsigned long long u64;
+constexpr int NT = 256, NW = NT / 64;
+constexpr int NV = 8;  // 16-byte vectors a thread holds
+constexpr int KMAX = 32;
+constexpr float LOG2E = 1.4426950408889634f;
+
+// 16 bytes at any element-aligned address
+typedef u32x4 __attribute__((aligned(2))) u32x4_any;
+
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  union {
+    u32x4 raw;
+    T e[N];
+  };
+  __device__ __forceinline__ float at(int i) const { return (float)e[i]; }
+};
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// values and places as one sortable word: larger value first, then the lower column
+__device__ __forceinline__ u64 order_key(float x, int col) {
+  const unsigned u = __float_as_uint(x + 0.f);  // -0 and +0 tie
+  const unsigned o = u ^ ((u >> 31) ? 0xffffffffu : 0x80000000u);
+  return ((u64)o << 32) | (unsigned)~col;
+}
+__device__ __forceinline__ int key_col(u64 k) { return (int)~(unsigned)k; }
+__device__ __forceinline__ float key_val(u64 k) {
+  const unsigned o = (unsigned)(k >> 32);
+  return __uint_as_float(o ^ ((o >> 31) ? 0x80000000u : 0xffffffffu));
+}
+__device__ __forceinline__ u64 wave_max64(u64 v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const u64 x = __shfl_xor(v, o, 64);
+    v = x > v ? x : v;
+  }
+  return v;
+}
+
+struct Stat {  // m, S, Y of a set of logits (m = -inf: none)
+  float m, s, y;
+};
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+  Stat r;
+  r.m = fmaxf(a.m, b.m);
+  // an empty side has s = y = 0; beyond e^-1e4 a side weighs nothing (and 0 * (inf) must not arise)
+  const float da = a.m == -INFINITY ? 0.f : fmaxf(a.m - r.m, -1e4f), db = b.m == -INFINITY ? 0.f : fmaxf(b.m - r.m, -1e4f);
+  const float ea = ex2(da * LOG2E), eb = ex2(db * LOG2E);
+  r.s = a.s * ea + b.s * eb;
+  r.y = (a.y + da * a.s) * ea + (b.y + db * b.s) * eb;
+  return r;
+}
+
+struct FwdParams {
+  const void* x;
+  const int* ids;
+  long long ld;
+  int V, T, k, ignore, parts, per;  // per: 16-byte vectors of a part
+  float *logp, *ent, *lse, *norm, *top_logp;  // norm [T][2]: m (-inf: no class), ln S
+  int* top_ids;
+  Stat* pstat;  // [T][parts]
+  u64* pkeys;   // [T][parts][k]
+};
+__device__ __forceinline__ float log_p(float x, float m, float ls) { return m == -INFINITY ? -INFINITY : (x - m) - ls; }
+template <typename T>
+__device__ __forceinline__ void write_row(const FwdParams& p, int row, const Stat& st) {
+  const bool any = !(st.s == 0.f);  // false: every logit is -inf
+  const float ls = any ? logf(st.s) : 0.f, m = any ? st.m : -INFINITY;
+  p.norm[2ll * row] = m;
+  p.norm[2ll * row + 1] = ls;
+  p.lse[row] = m + ls;
+  p.ent[row] = any ? ls - st.y / st.s : 0.f;
+  const int id = p.ids[row];
+  const bool use = id != p.ignore && (unsigned)id < (unsigned)p.V;
+  p.logp[row] = use ? log_p((float)((const T*)p.x)[(long long)row * p.ld + id], m, ls) : 0.f;
+}
+__device__ __forceinline__ void write_top(const FwdParams& p, int row, int j, u64 key, const Stat& st, float ls) {
+  p.top_ids[(long long)row * p.k + j] = key_col(key);
+  p.top_logp[(long long)row * p.k + j] = st.s == 0.f ? -INFINITY : log_p(key_val(key), st.m, ls);
+}
+
+template <typename T>
+__device__ __forceinline__ void load_vec(Vec<T>& v, const T* x, int i, int V) {
+  constexpr int N = Vec<T>::N;
+  if ((i + 1) * N <= V) {
+    v.raw = *(const u32x4_any*)(x + i * N);
+  } else {
+#pragma unroll
+    for (int e = 0; e < N; ++e) v.e[e] = i * N + e < V ? x[i * N + e] : (T)-INFINITY;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(NT) void logprobs_fwd_kernel(FwdParams p) {
+  constexpr int N = Vec<T>::N;
+  __shared__ Stat wst[NW];
+  __shared__ u64 wkey[2][NW];
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const T* x = (const T*)p.x + (long long)row * p.ld;
+  const int nvec = (p.V + N - 1) / N, v0 = part * p.per, v1 = min(nvec, v0 + p.per);
+  Vec<T> v[NV];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int i = v0 + c * NT + (int)threadIdx.x;
+    if (i < v1) {
+      load_vec<T>(v[c], x, i, p.V);
+    } else {
+#pragma unroll
+      for (int e = 0; e < N; ++e) v[c].e[e] = (T)-INFINITY;
+    }
+  }
+  float m = -INFINITY;
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int e = 0; e < N; ++e) m = fmaxf(m, v[c].at(e));
+  Stat st;
+  st.m = wave_max(m);
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  st.s = st.y = 0.f;
+#pragma unroll
+  for (int c = 0; c < NV; ++c)
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float d = v[c].at(e) - ref;
+      const float ee = ex2(d * LOG2E);
+      st.s += ee;
+      st.y = fmaf(fmaxf(d, -1e30f), ee, st.y);  // -inf: 0 * -1e30, not 0 * -inf
+    }
+  st.s = wave_sum(st.s);
+  st.y = wave_sum(st.y);
+  if (l == 0) wst[w] = st;
+  __syncthreads();
+  st = wst[0];
+#pragma unroll
+  for (int u = 1; u < NW; ++u) st = join(st, wst[u]);
+  if (threadIdx.x == 0) {
+    if (p.parts == 1) write_row<T>(p, row, st);
+    else p.pstat[(long long)row * p.parts + part] = st;
+  }
+  if (p.k == 0) return;
+  const float ls = st.s == 0.f ? 0.f : logf(st.s);
+  // the k best, one after another: each round takes the largest key below the last one
+  u64 prev = ~0ull;
+  for (int j = 0; j < p.k; ++j) {
+    u64 best = 0;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int col = (v0 + c * NT + (int)threadIdx.x) * N + e;
+        const u64 key = col < min(p.V, v1 * N) ? order_key(v[c].at(e), col) : 0;
+        best = key < prev && key > best ? key : best;
+      }
+    best = wave_max64(best);
+    if (l == 0) wkey[j & 1][w] = best;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NW; ++u) best = wkey[j & 1][u] > best ? wkey[j & 1][u] : best;
+    prev = best;
+    if (threadIdx.x == 0) {
+      if (p.parts == 1) write_top(p, row, j, best, st, ls);
+      else p.pkeys[((long long)row * p.parts + part) * p.k + j] = best;
+    }
+  }
+}
+
+// one block per row: joins its parts; the k best of parts * k candidates by counting the larger ones
+template <typename T>
+__global__ __launch_bounds__(64) void logprobs_join_kernel(FwdParams p) {
+  const int row = blockIdx.x;
+  const Stat* ps = p.pstat + (long long)row * p.parts;
+  Stat st = ps[0];
+  for (int u = 1; u < p.parts; ++u) st = join(st, ps[u]);
+  if (threadIdx.x == 0) write_row<T>(p, row, st);
+  if (p.k == 0) return;
+  const float ls = st.s == 0.f ? 0.f : logf(st.s);
+  const u64* pk = p.pkeys + (long long)row * p.parts * p.k;
+  const int n = p.parts * p.k;
+  for (int i = threadIdx.x; i < n; i += 64) {
+    const u64 key = pk[i];
+    int r = 0;
+    for (int j = 0; j < n; ++j) r += pk[j] > key ? 1 : 0;
+    if (key != 0 && r < p.k) write_top(p, row, r, key, st, ls);
+  }
+}
+
+struct BwdParams {
+  const void* x;
+  void* dx;
+  const int *ids, *top_ids;
+  long long ld, ldd;
+  int V, T, k, ignore, parts, per, cols;  // cols: columns of dx, V..cols-1 get zeros
+  const float *norm, *ent, *dlogp, *dent, *dtop;
+};
+template <typename T>
+__global__ __launch_bounds__(NT) void logprobs_bwd_kernel(BwdParams p) {
+  constexpr int N = Vec<T>::N;
+  const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
+  const T* x = (const T*)p.x + (long long)row * p.ld;
+  T* d = (T*)p.dx + (long long)row * p.ldd;
+  const int nvec = (p.cols + N - 1) / N, v0 = part * p.per, v1 = min(nvec, v0 + p.per);
+  Vec<T> v[NV];
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int i = v0 + c * NT + (int)threadIdx.x;
+    if (i < v1 && i * N < p.V) load_vec<T>(v[c], x, i, p.V);
+  }
+  const int id = p.ids[row];
+  const bool use = id != p.ignore && (unsigned)id < (unsigned)p.V;
+  const float gl = use && p.dlogp ? p.dlogp[row] : 0.f;
+  const float gh = p.dent ? p.dent[row] : 0.f;
+  float tot = gl;
+  for (int j = 0; j < p.k; ++j) tot += p.dtop[(long long)row * p.k + j];
+  const float m = p.norm[2ll * row], ls = p.norm[2ll * row + 1], ent = p.ent[row];
+  auto grad = [&](float xv) {  // the part every column has
+    const float lp = fmaxf(log_p(xv, m, ls), -1e4f);  // p = 0 there
+    const float pr = ex2(lp * LOG2E);
+    return -pr * fmaf(gh, lp + ent, tot);
+  };
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    const int i = v0 + c * NT + (int)threadIdx.x;
+    if (i < v1) {
+      Vec<T> o;
+#pragma unroll
+      for (int e = 0; e < N; ++e) o.e[e] = (T)(i * N + e < p.V ? grad(v[c].at(e)) : 0.f);
+      if ((i + 1) * N <= p.cols) {
+        *(u32x4_any*)(d + i * N) = o.raw;
+      } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e)
+          if (i * N + e < p.cols) d[i * N + e] = o.e[e];
+      }
+    }
+  }
+  // the named columns once more, with their own terms (after this block's plain stores)
+  __syncthreads();
+  if ((int)threadIdx.x <= p.k) {
+    const int col = threadIdx.x == 0 ? id : p.top_ids[(long long)row * p.k + threadIdx.x - 1];
+    if ((threadIdx.x > 0 || use) && (unsigned)col < (unsigned)p.V && col >= v0 * N && col < v1 * N) {
+      float g = use && col == id ? gl : 0.f;
+      for (int j = 0; j < p.k; ++j)
+        if (p.top_ids[(long long)row * p.k + j] == col) g += p.dtop[(long long)row * p.k + j];
+      d[col] = (T)(g + grad((float)x[col]));
+    }
+  }
+}
+
+// parts of a row and the vectors of each: at most NT * NV of them, even shares
+void cut(int vecs, int& parts, int& per) {
+  parts = (vecs + NT * NV - 1) / (NT * NV);
+  per = (vecs + parts - 1) / parts;
+}
+int vecs_of(int cols, int dtype) { const int n = dtype == 2 ? 4 : 8; return (cols + n - 1) / n; }
+}  // namespace
+
+extern "C" {
+int tfk_logprobs_kmax() { return KMAX; }
+// bytes of workspace of a forward (0: none)
+long long tfk_logprobs_ws(long long T, int V, int dtype, int k) {
+  int parts, per;
+  cut(vecs_of(V, dtype), parts, per);
+  return parts == 1 ? 0 : T * parts * (16 + 8ll * k);
+}
+// dtype: 0 bf16, 1 f16, 2 f32
+int tfk_logprobs_fwd(const void* x, int dtype, const int* ids, int T, int V, long long ld, int k, int ignore, float* logp,
+                     float* ent, float* lse, float* norm, float* top_logp, int* top_ids, void* ws, hipStream_t s) {
+  if (T <= 0) return 0;
+  FwdParams p{x, ids, ld, V, T, k, ignore, 0, 0, logp, ent, lse, norm, top_logp, top_ids, nullptr, nullptr};
+  cut(vecs_of(V, dtype), p.parts, p.per);
+  p.pkeys = (u64*)ws;
+  p.pstat = (Stat*)((u64*)ws + (long long)T * p.parts * k);
+  const dim3 g((unsigned)((long long)T * p.parts));
+#define TFK_LP(T_)                                                                       \
+  hipLaunchKernelGGL(logprobs_fwd_kernel<T_>, g, dim3(NT), 0, s, p);                      \
+  if (p.parts > 1) hipLaunchKernelGGL(logprobs_join_kernel<T_>, dim3(T), dim3(64), 0, s, p);
+  if (dtype == 0) { TFK_LP(bf16) } else if (dtype == 1) { TFK_LP(f16) } else { TFK_LP(float) }
+#undef TFK_LP
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+// dx: cols >= V columns, row stride ldd; dlogp / dent may be null; k = 0: no alternatives
+int tfk_logprobs_bwd(const void* x, int dtype, const int* ids, int T, int V, long long ld, int k, int ignore,
+                     const float* norm, const float* ent, const int* top_ids, const float* dlogp, const float* dent,
+                     const float* dtop, void* dx, long long ldd, int cols, hipStream_t s) {
+  if (T <= 0) return 0;
+  BwdParams p{x, dx, ids, top_ids, ld, ldd, V, T, k, ignore, 0, 0, cols, norm, ent, dlogp, dent, dtop};
+  cut(vecs_of(cols, dtype), p.parts, p.per);
+  const dim3 g((unsigned)((long long)T * p.parts));
+  if (dtype == 0) hipLaunchKernelGGL(logprobs_bwd_kernel<bf16>, g, dim3(NT), 0, s, p);
+  else if (dtype == 1) hipLaunchKernelGGL(logprobs_bwd_kernel<f16>, g, dim3(NT), 0, s, p);
+  else hipLaunchKernelGGL(logprobs_bwd_kernel<float>, g, dim3(NT), 0, s, p);
+  return hipGetLastError() == hipSuccess ? 0 : -1;
+}
+}

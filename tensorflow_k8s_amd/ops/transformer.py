@@ -4,6 +4,11 @@ multi-head attention. bf16 activations, f32 statistics/gradients of parameters.
 Attention operands are *column views* of 2-D token-major buffers: ``(buf, col)`` means the
 [B*S, H*64] block of ``buf[:, col:col + H*64]`` -- e.g. q/k/v straight out of a fused QKV
 projection ``qkv[B*S, 3*H*64]`` (q at col 0, k at H*64, v at 2*H*64). No head transposes.
+
+Attention with shaped scores (csrc/kernels/attn_shaped.hip) is the same AttnSpec with any of softcap,
+slopes, docs, prefix_len, q_start, kv_heads or head_dim given: document and prefix masks, a tanh cap,
+a bias by distance, query heads that share key heads, queries at a position of a longer key sequence.
+The embedding gradient by sorted tokens (csrc/kernels/embed_sort.hip) is token_order + embedding_bwd_sorted.
 CPU paths are fp32 references with the same rounding points and (for dropout) the same hash RNG.
 """
 from __future__ import annotations
@@ -162,6 +167,56 @@ def embedding_bwd(ids, dy, dword, dpos=None, seq_len: int = 1, type_ids=None, dt
     lib().embedding_bwd(ids, dy, dword, dpos, seq_len, type_ids, dtype_table, W, scale)
 
 
+class TokenOrder:
+    """Token positions in the order of their ids (token_order): perm int32 [T], the stable sort of the
+    positions by id; keys int32 [T], the sorted ids, padding (ids outside [0, V)) as V at the end."""
+
+    def __init__(self, V: int, perm: torch.Tensor, keys: torch.Tensor):
+        self.V, self.perm, self.keys = V, perm, keys
+
+
+def token_order(ids: torch.Tensor, V: int) -> TokenOrder:
+    """The order in which embedding_bwd_sorted sums the gradient rows of ids (int32, any shape): one
+    order serves every table that is indexed by the same ids. It depends on the ids alone (no host
+    synchronisation, same result from run to run)."""
+    if ids.dtype != torch.int32:
+        raise TypeError(f"token_order: ids must be int32, got {ids.dtype}")
+    if V < 1:
+        raise ValueError(f"token_order: V must be at least 1, got {V}")
+    flat = ids.reshape(-1).contiguous()
+    if not on_gpu(ids):
+        key = torch.where((flat >= 0) & (flat < V), flat, V)
+        keys, perm = torch.sort(key, stable=True)
+        return TokenOrder(V, perm.to(torch.int32), keys.to(torch.int32))
+    perm, keys = torch.empty_like(flat), torch.empty_like(flat)
+    lib().token_order(flat, V, perm, keys)
+    return TokenOrder(V, perm, keys)
+
+
+def embedding_bwd_sorted(order: TokenOrder, dy: torch.Tensor, dword: torch.Tensor, scale: float = 1.0,
+                         accumulate: bool = True) -> None:
+    """dword[r] (+)= scale * sum of the dy rows of the tokens with id r, for r < order.V; tokens with ids
+    outside the table add nothing. dword f32 [order.V, W]; dy bf16 / f16 / f32 [..., W] (rows may be
+    strided). Sums run in f32 in the tokens' order and use no atomics, so results are bitwise the same
+    from run to run. accumulate=False writes every row, zeros where no token has the id. (embedding_bwd
+    sums a row's tokens in no fixed order.)"""
+    W = dword.shape[-1]
+    if dword.dim() != 2 or dword.shape[0] != order.V:
+        raise ValueError(f"embedding_bwd_sorted: dword must be [{order.V}, W], got {tuple(dword.shape)}")
+    T = order.perm.numel()
+    if dy.shape[-1] != W or dy.numel() != T * W:
+        raise ValueError(f"embedding_bwd_sorted: dy must be [{T}, {W}], got {tuple(dy.shape)}")
+    if dy.dim() != 2:
+        dy = dy.reshape(T, W)
+    if not on_gpu(dy):
+        if not accumulate:
+            dword.zero_()
+        use = order.keys < order.V
+        dword.index_add_(0, order.keys[use].long(), dy.float()[order.perm[use].long()] * scale)
+        return
+    lib().embedding_bwd_sorted(order.perm, order.keys, dy, dword, scale, accumulate)
+
+
 # ----------------------------------------------------------------------------- attention
 
 def gather_rows(src: torch.Tensor, pos: torch.Tensor | None, S: int) -> torch.Tensor:
@@ -250,14 +305,84 @@ def _ref_probs(q, k, kv_len, causal, scale):
     return torch.softmax(s, -1).nan_to_num(0.0)
 
 
-class AttnSpec:
-    """Geometry of one attention call: q/k/v column views of token-major buffers."""
+def document_spans(doc_ids: torch.Tensor) -> torch.Tensor:
+    """Document mask of packed rows for AttnSpec(docs=...): doc_ids int32 [B, S] -> int32 [B, S, 2], the
+    first position and the end of the run of equal ids around each token; (0, 0) where the id is negative
+    (padding: sees nothing, is seen by nothing). A document is a RUN of equal ids: an id that comes
+    again after another one starts a new document. Made once per batch, used by every layer."""
+    if doc_ids.dtype != torch.int32 or doc_ids.dim() != 2:
+        raise TypeError(f"document_spans: ids must be int32 [B, S], got {doc_ids.dtype} {tuple(doc_ids.shape)}")
+    B, S = doc_ids.shape
+    if on_gpu(doc_ids):
+        out = torch.empty(B, S, 2, dtype=torch.int32, device=doc_ids.device)
+        lib().doc_spans(doc_ids.contiguous(), out)
+        return out
+    new = torch.ones(B, S, dtype=torch.bool)
+    new[:, 1:] = doc_ids[:, 1:] != doc_ids[:, :-1]
+    i = torch.arange(S).expand(B, S)
+    first = torch.where(new, i, 0).cummax(1).values
+    last = torch.ones(B, S, dtype=torch.bool)
+    last[:, :-1] = new[:, 1:]
+    end = torch.where(last, i + 1, S).flip(1).cummin(1).values.flip(1)
+    return torch.where((doc_ids >= 0)[..., None], torch.stack([first, end], -1), 0).to(torch.int32)
 
-    def __init__(self, B, H, Sq, Sk, q, k, v, kv_len=None, causal=False, p_drop=0.0, seed=0, scale=None):
+
+class AttnSpec:
+    """Geometry of one attention call: q/k/v column views of token-major buffers.
+
+    Shaped scores (any of the keyword arguments below; bf16 or f16, head_dim 64 or 128):
+      score(i, j) = softcap tanh(scale q_i.k_j / softcap) - slopes[h] |p_i - j|
+    kv_heads    key/value heads; query heads h G .. h G + G - 1 (G = H / kv_heads) share key head h
+    softcap     > 0: tanh cap of the scaled scores
+    slopes      f32 [H]: bias by distance (constants: no gradient)
+    q_start     int32 [B]: query i of batch b stands at key position p_i = i + q_start[b] (default 0)
+    prefix_len  int32 [B], with causal: keys below it are seen by every query, else key j by p_i >= j
+    docs        document_spans of the key sequence: a query at position p sees its own document only
+                (positions outside the sequence see nothing)
+    kv_len, causal, p_drop and seed as in the plain form (causal compares with p_i). A query that sees
+    no key has output 0, lse +inf and no gradient. Keys that no query of the call can see (beyond kv_len,
+    padding of docs, outside the walked range) may hold anything; a non-finite value in a key that some
+    queries see can reach the others of the same tile. Buffers may be 2-D [B*S, width] or 3-D [B, S', width]
+    with S' >= S (a cache with room), rows any multiple of 8 elements apart."""
+
+    def __init__(self, B, H, Sq, Sk, q, k, v, kv_len=None, causal=False, p_drop=0.0, seed=0, scale=None, *,
+                 kv_heads=None, head_dim=HEAD_DIM, softcap=0.0, slopes=None, docs=None, prefix_len=None,
+                 q_start=None):
         self.B, self.H, self.Sq, self.Sk = B, H, Sq, Sk
         self.q, self.k, self.v = q, k, v  # (buf, col)
         self.kv_len, self.causal, self.p_drop, self.seed = kv_len, causal, p_drop, seed
-        self.scale = scale if scale is not None else 1.0 / math.sqrt(HEAD_DIM)
+        self.head_dim, self.kv_heads = head_dim, H if kv_heads is None else kv_heads
+        self.scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
+        self.softcap, self.slopes, self.docs = float(softcap or 0.0), slopes, docs
+        self.prefix_len, self.q_start = prefix_len, q_start
+        self.shaped = (self.softcap != 0.0 or slopes is not None or docs is not None or prefix_len is not None
+                       or q_start is not None or self.kv_heads != H or head_dim != HEAD_DIM
+                       or q[0].dtype == torch.float16 or any(b.dim() == 3 for b, _ in (q, k, v)))
+        if self.shaped:
+            self._check()
+
+    def _check(self):
+        if self.head_dim not in (64, 128):
+            raise ValueError(f"attention: head_dim must be 64 or 128, got {self.head_dim}")
+        if self.kv_heads < 1 or self.H % self.kv_heads:
+            raise ValueError(f"attention: {self.H} heads do not share {self.kv_heads} key heads evenly")
+        if min(self.B, self.Sq, self.Sk) < 1:
+            raise ValueError(f"attention: empty shape B={self.B} Sq={self.Sq} Sk={self.Sk}")
+        if not (math.isfinite(self.softcap) and self.softcap >= 0.0):
+            raise ValueError(f"attention: softcap must be >= 0, got {self.softcap}")
+        if not (math.isfinite(self.scale) and self.scale > 0.0):
+            raise ValueError(f"attention: scale must be positive, got {self.scale}")
+        if self.prefix_len is not None and not self.causal:
+            raise ValueError("attention: prefix_len needs causal=True")
+        for n, t, dt, shape in (("kv_len", self.kv_len, torch.int32, (self.B,)), ("q_start", self.q_start, torch.int32, (self.B,)),
+                                ("prefix_len", self.prefix_len, torch.int32, (self.B,)),
+                                ("slopes", self.slopes, torch.float32, (self.H,)),
+                                ("docs", self.docs, torch.int32, (self.B, self.Sk, 2))):
+            if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()):
+                raise ValueError(f"attention: {n} must be contiguous {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
+        for n, (buf, col), S, heads in (("q", self.q, self.Sq, self.H), ("k", self.k, self.Sk, self.kv_heads),
+                                        ("v", self.v, self.Sk, self.kv_heads)):
+            _span_check(n, buf, col, self.B, S, heads * self.head_dim)
 
     def strides(self):
         out = []
@@ -267,8 +392,105 @@ class AttnSpec:
         return out
 
 
+def _span_check(n, buf, col, B, S, W):
+    """A (buf, col) operand of shaped attention holds [B, S, W] at column col."""
+    if buf.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"attention: {n} must be bfloat16 or float16, got {buf.dtype}")
+    ok = (buf.dim() == 2 and buf.shape[0] == B * S) or (buf.dim() == 3 and buf.shape[0] == B and buf.shape[1] >= S)
+    if not ok or col < 0 or col + W > buf.shape[-1]:
+        raise ValueError(f"attention: {n} must hold [{B}*{S}, {W}] at column {col}, got {list(buf.shape)}")
+
+
+def _buf_strides(buf, S):
+    """[batch, token] strides of a 2-D [B*S, width] or 3-D [B, S', width] buffer."""
+    return [buf.stride(0), buf.stride(1)] if buf.dim() == 3 else [S * buf.stride(0), buf.stride(0)]
+
+
+def _shaped_view(buf, col, B, S, heads, D):
+    """[B, S, heads, D] view of a (buf, col) operand."""
+    x = buf[:, :S] if buf.dim() == 3 else buf.unflatten(0, (B, S))
+    return x[..., col:col + heads * D].unflatten(-1, (heads, D))
+
+
+def _shaped_ref(sp, q, k, v):
+    """f32 reference of shaped attention on q [B,Sq,H,D], k, v [B,Sk,Hk,D] -> (out, lse)."""
+    B, H, Sq, Sk, G = sp.B, sp.H, sp.Sq, sp.Sk, sp.H // sp.kv_heads
+    k, v = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
+    s = torch.einsum("bqhd,bkhd->bhqk", q, k) * sp.scale
+    if sp.softcap:
+        s = sp.softcap * torch.tanh(s / sp.softcap)
+    j = torch.arange(Sk)
+    p = torch.arange(Sq)[None, :] + (sp.q_start.long()[:, None] if sp.q_start is not None else torch.zeros(B, 1, dtype=torch.long))
+    if sp.slopes is not None:
+        s = s - sp.slopes[None, :, None, None] * (p[:, :, None] - j).abs()[:, None]
+    ok = torch.ones(B, Sq, Sk, dtype=torch.bool)
+    if sp.causal:
+        ok = j <= p[:, :, None]
+        if sp.prefix_len is not None:
+            ok = ok | (j < sp.prefix_len.long()[:, None, None])
+    if sp.kv_len is not None:
+        ok = ok & (j < sp.kv_len.long()[:, None, None])
+    if sp.docs is not None:
+        d = torch.gather(sp.docs.long(), 1, p.clamp(0, Sk - 1)[..., None].expand(B, Sq, 2))
+        inside = (p >= 0) & (p < Sk)
+        ok = ok & inside[:, :, None] & (j >= d[..., :1]) & (j < d[..., 1:])
+    ok = ok[:, None]
+    s = s.masked_fill(~ok, float("-inf"))
+    m = s.amax(-1, keepdim=True)
+    e = torch.exp(s - m.masked_fill(m == float("-inf"), 0.0))
+    l = e.sum(-1, keepdim=True)
+    lse = torch.where(l > 0, m + torch.log(l), float("inf"))[..., 0]
+    pr = e / l.masked_fill(l == 0, 1.0)
+    if sp.p_drop > 0:
+        pr = pr * dropout_keep_mask(eff_seed(sp.seed), B, H, Sq, Sk, sp.p_drop) * attn_keep_scale(sp.p_drop)
+    # keys that no query of the batch sees may hold anything
+    v = torch.where(ok[:, 0].any(1)[:, :, None, None], v, 0.0)
+    return torch.einsum("bhqk,bkhd->bqhd", pr, v), lse
+
+
+def _shaped_args(sp):
+    return [sp.kv_len, sp.q_start, sp.prefix_len, sp.docs, sp.slopes, sp.scale, sp.softcap, sp.causal, sp.p_drop, sp.seed]
+
+
+def _shaped_fwd(sp):
+    B, H, Sq, Sk, Hk, D = sp.B, sp.H, sp.Sq, sp.Sk, sp.kv_heads, sp.head_dim
+    q = sp.q[0]
+    if not on_gpu(q):
+        o, lse = _shaped_ref(sp, *(_shaped_view(b, c, B, S, n, D).float() for (b, c), S, n in
+                                   ((sp.q, Sq, H), (sp.k, Sk, Hk), (sp.v, Sk, Hk))))
+        return o.reshape(B * Sq, H * D).to(q.dtype), lse
+    out = torch.empty(B * Sq, H * D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=q.device)
+    st = _buf_strides(q, Sq) + _buf_strides(sp.k[0], Sk) + _buf_strides(sp.v[0], Sk) + [Sq * H * D, H * D]
+    lib().shaped_fwd(q, sp.q[1], sp.k[0], sp.k[1], sp.v[0], sp.v[1], out, lse, [B, H, Hk, Sq, Sk, D], st, *_shaped_args(sp))
+    return out, lse
+
+
+def _shaped_bwd(sp, out, dout, lse, dq, dk, dv):
+    B, H, Sq, Sk, Hk, D = sp.B, sp.H, sp.Sq, sp.Sk, sp.kv_heads, sp.head_dim
+    dout = dout.reshape(B * Sq, H * D)
+    geom = ((sp.q, dq, Sq, H), (sp.k, dk, Sk, Hk), (sp.v, dv, Sk, Hk))
+    for n, (_, (buf, col), S, heads) in zip(("dq", "dk", "dv"), geom):
+        _span_check(n, buf, col, B, S, heads * D)
+    if not on_gpu(out):
+        ins = [_shaped_view(b, c, B, S, n, D).float().requires_grad_(True) for (b, c), _, S, n in geom]
+        with torch.enable_grad():
+            o, _ = _shaped_ref(sp, *ins)
+            grads = torch.autograd.grad(o, ins, dout.float().reshape(B, Sq, H, D))
+        for (_, (buf, col), S, n), g in zip(geom, grads):
+            _shaped_view(buf, col, B, S, n, D).copy_(g.to(buf.dtype))
+        return
+    dout = dout.contiguous()
+    st = _buf_strides(sp.q[0], Sq) + _buf_strides(sp.k[0], Sk) + _buf_strides(sp.v[0], Sk) + [Sq * H * D, H * D]
+    gst = _buf_strides(dq[0], Sq) + _buf_strides(dk[0], Sk) + _buf_strides(dv[0], Sk)
+    lib().shaped_bwd(sp.q[0], sp.q[1], sp.k[0], sp.k[1], sp.v[0], sp.v[1], out, dout, lse, dq[0], dq[1], dk[0], dk[1],
+                     dv[0], dv[1], [B, H, Hk, Sq, Sk, D], st, gst, *_shaped_args(sp))
+
+
 def attention_fwd(sp: AttnSpec):
-    """Returns (out bf16 [B*Sq, H*64], lse f32 [B,H,Sq])."""
+    """Returns (out bf16 [B*Sq, H*64], lse f32 [B,H,Sq]) (shaped: out in q's type, [B*Sq, H*head_dim])."""
+    if sp.shaped:
+        return _shaped_fwd(sp)
     B, H, Sq, Sk = sp.B, sp.H, sp.Sq, sp.Sk
     dev = sp.q[0].device
     if not on_gpu(sp.q[0]):
@@ -290,6 +512,8 @@ def attention_fwd(sp: AttnSpec):
 
 def attention_bwd(sp: AttnSpec, out, dout, lse, dq, dk, dv):
     """dq/dk/dv: (buf, col) views to write (e.g. column slices of a fused dQKV buffer)."""
+    if sp.shaped:
+        return _shaped_bwd(sp, out, dout, lse, dq, dk, dv)
     B, H, Sq, Sk = sp.B, sp.H, sp.Sq, sp.Sk
     if not on_gpu(out):
         q, k, v = (_view(b, c, B, S, H).float().requires_grad_(True)
