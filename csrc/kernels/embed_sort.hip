@@ -6,7 +6,7 @@
 // every sum below has a fixed order of its terms: no float atomics, equal bits from run to run.
 //
 // Gradient: dword[r] (+)= scale * sum over the positions t with ids[t] == r of dy[t], in f32. The
-// sorted positions are cut into chunks of CHUNK; a group of lanes (8 columns each) walks a chunk and
+// sorted positions are cut into chunks (chunk_of); a group of lanes (8 columns each) walks a chunk and
 // sums each run of equal keys. A run inside one chunk is written at once; the pieces of a run that
 // crosses a chunk border go to a workspace (`part`: a head and a tail row per chunk) and a second
 // launch adds them in chunk order, so a token that fills half the batch is summed by many groups.
@@ -18,36 +18,62 @@ namespace {
 typedef _Float16 f16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int NT = 256;
-constexpr int CHUNK = 32;
 
 __device__ __forceinline__ int key_of(int id, int V) { return (unsigned)id < (unsigned)V ? id : V; }
 
 // ------------------------------------------------------------------------------- order by counting
-// rank(i) = #{j : key_j < key_i} + #{j < i : key_j == key_i}, one launch. T^2 compares: a wave holds
-// 64 positions, the 16 waves of a block share them and divide the j's, the counts meet in LDS.
+// rank(i) = #{j : key_j < key_i} + #{j < i : key_j == key_i}, one launch. T^2 compares: a block holds 32
+// positions (one a lane of each half wave), its 16 waves divide the j's, the two halves of a wave take
+// alternate groups of 16 j's, and the counts meet in LDS. A wave stages its j's keys in LDS and reads
+// them back four at a time, the same for all lanes of a half, so a compare is two vector instructions:
+// key_j < key_i + 1 for the j's before the block's positions, key_j < key_i for those behind.
+// 8192 tokens: 8 us (scalar loads of the keys, 64 positions a block: 21 us, one load's latency per 16 keys).
+constexpr int STAGE = 512, OP = 32;
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 __global__ __launch_bounds__(1024) void order_count_kernel(const int* __restrict__ ids, int T, int V,
                                                            int* __restrict__ perm, int* __restrict__ keys) {
-  __shared__ int cnt[16][64];
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int i = blockIdx.x * 64 + l;
+  __shared__ int cnt[32][OP];
+  __shared__ __attribute__((aligned(16))) int stage[16][STAGE];
+  const int l = threadIdx.x & 63, hw = l >> 5, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i0 = blockIdx.x * OP, i = i0 + (l & 31);
   const int key = key_of(ids[min(i, T - 1)], V);
-  const int per = (T + 15) / 16, j0 = w * per, j1 = min(T, j0 + per);
+  const int per = ((T + 15) / 16 + 3) & ~3, j0 = w * per, j1 = min(T, j0 + per);
   int n = 0;
-  for (int j = j0; j < j1; j += 64) {
-    // the wave's 64 keys, broadcast lane by lane
-    const int kj = j + l < j1 ? key_of(ids[j + l], V) : 0x7fffffff;
-    const int m = min(64, j1 - j);
-    for (int e = 0; e < m; ++e) {
-      const int k = __builtin_amdgcn_readlane(kj, e);
-      n += (k < key || (k == key && j + e < i)) ? 1 : 0;
+  for (int g0 = j0; g0 < j1; g0 += STAGE) {
+    const int m = min(STAGE, j1 - g0);
+    int v[STAGE / 64];
+#pragma unroll
+    for (int u = 0; u < STAGE / 64; ++u) v[u] = ids[min(g0 + u * 64 + l, T - 1)];
+#pragma unroll
+    for (int u = 0; u < STAGE / 64; ++u) stage[w][u * 64 + l] = u * 64 + l < m ? key_of(v[u], V) : 0x7fffffff;
+    __builtin_amdgcn_wave_barrier();  // the wave's own buffer: its LDS operations are in order
+#pragma unroll 2
+    for (int q0 = 0; q0 < m; q0 += 32) {
+      const int q = q0 + 16 * hw, j = g0 + q;
+      i32x4 k[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) k[u] = *(const i32x4*)&stage[w][q + 4 * u];
+      if (g0 + q0 + 32 <= i0 || g0 + q0 >= i0 + OP) {
+        const int lim = key + (g0 + q0 < i0 ? 1 : 0);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n += k[u][e] < lim ? 1 : 0;
+      } else {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) n += k[u][e] < key + (j + 4 * u + e < i ? 1 : 0) ? 1 : 0;
+      }
     }
+    __builtin_amdgcn_wave_barrier();
   }
-  cnt[w][l] = n;
+  cnt[2 * w + hw][l & 31] = n;
   __syncthreads();
-  if (w == 0 && i < T) {
+  if (threadIdx.x < OP && i < T) {
     int r = 0;
 #pragma unroll
-    for (int u = 0; u < 16; ++u) r += cnt[u][l];
+    for (int u = 0; u < 32; ++u) r += cnt[u][threadIdx.x];
     perm[r] = i;
     keys[r] = key;
   }
@@ -80,21 +106,27 @@ template <bool FIRST>
 __global__ __launch_bounds__(RT) void radix_place_kernel(const int* __restrict__ src, const int* __restrict__ psrc, int T,
                                                          int V, int shift, int bits, const int* __restrict__ hist,
                                                          int* __restrict__ dst, int* __restrict__ pdst) {
+  constexpr int DPT = (1 << RB_MAX) / RT, IPL = RTILE / RW / 64;  // digits of a thread, items of a lane
   __shared__ int at[RW][1 << RB_MAX];  // next place of (wave, digit)
-  __shared__ int tot[RT];
+  __shared__ int tot[RW];
   const int nd = 1 << bits, nb = gridDim.x, l = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int d = threadIdx.x; d < nd * RW; d += RT) at[d / nd][d % nd] = 0;
-  __syncthreads();
-  const int w0 = blockIdx.x * RTILE + w * (RTILE / RW), w1 = min(T, w0 + RTILE / RW);
-  for (int i = w0 + l; i < w1; i += 64) atomicAdd(&at[w][(radix_key<FIRST>(src, i, V) >> shift) & (nd - 1)], 1);
+  const int w0 = blockIdx.x * RTILE + w * (RTILE / RW);
+  int k[IPL], v[IPL];
+#pragma unroll
+  for (int u = 0; u < IPL; ++u) {
+    const int i = min(w0 + u * 64 + l, T - 1);
+    k[u] = radix_key<FIRST>(src, i, V);
+    v[u] = FIRST ? i : psrc[i];
+  }
   // digits d0 .. d0 + per - 1 belong to this thread: items of smaller digits anywhere, then of equal
   // digits in earlier tiles
   const int per = (nd + RT - 1) / RT, d0 = threadIdx.x * per;
-  int all[(1 << RB_MAX) / RT], before[(1 << RB_MAX) / RT], mine = 0;
+  int all[DPT], before[DPT], mine = 0;
 #pragma unroll
-  for (int u = 0; u < (1 << RB_MAX) / RT; ++u) {
+  for (int u = 0; u < DPT; ++u) {
     all[u] = before[u] = 0;
     if (u < per && d0 + u < nd) {
+#pragma unroll 16
       for (int b = 0; b < nb; ++b) {
         const int c = hist[(long long)b * nd + d0 + u];
         all[u] += c;
@@ -103,33 +135,39 @@ __global__ __launch_bounds__(RT) void radix_place_kernel(const int* __restrict__
       mine += all[u];
     }
   }
-  tot[threadIdx.x] = mine;
+  for (int d = threadIdx.x; d < nd * RW; d += RT) at[d / nd][d % nd] = 0;
   __syncthreads();
-  for (int o = 1; o < RT; o <<= 1) {  // inclusive scan of the threads' totals
-    const int v = threadIdx.x >= o ? tot[threadIdx.x - o] : 0;
-    __syncthreads();
-    tot[threadIdx.x] += v;
-    __syncthreads();
-  }
-  int base = tot[threadIdx.x] - mine;
 #pragma unroll
-  for (int u = 0; u < (1 << RB_MAX) / RT; ++u)
+  for (int u = 0; u < IPL; ++u)
+    if (w0 + u * 64 + l < T) atomicAdd(&at[w][(k[u] >> shift) & (nd - 1)], 1);
+  int base = mine;  // inclusive scan over the block: within the wave, then over the waves' totals
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int x = __shfl_up(base, o, 64);
+    base += l >= o ? x : 0;
+  }
+  if (l == 63) tot[w] = base;
+  __syncthreads();
+  base -= mine;
+  for (int u = 0; u < w; ++u) base += tot[u];
+#pragma unroll
+  for (int u = 0; u < DPT; ++u)
     if (u < per && d0 + u < nd) {
       int p = base + before[u];
-      for (int v = 0; v < RW; ++v) {
-        const int c = at[v][d0 + u];
-        at[v][d0 + u] = p;
+#pragma unroll
+      for (int x = 0; x < RW; ++x) {
+        const int c = at[x][d0 + u];
+        at[x][d0 + u] = p;
         p += c;
       }
       base += all[u];
     }
   __syncthreads();
   // items in order: equal digits of one 64-item round by a match over the digit's bits
-  for (int i0 = w0; i0 < w1; i0 += 64) {
-    const int i = i0 + l;
-    const bool ok = i < w1;
-    const int k = ok ? radix_key<FIRST>(src, i, V) : 0;
-    const int d = (k >> shift) & (nd - 1);
+#pragma unroll
+  for (int u = 0; u < IPL; ++u) {
+    const bool ok = w0 + u * 64 + l < T;
+    const int d = (k[u] >> shift) & (nd - 1);
     unsigned long long same = __ballot(ok);
     for (int b = 0; b < bits; ++b) {
       const unsigned long long m = __ballot((d >> b) & 1);
@@ -142,8 +180,8 @@ __global__ __launch_bounds__(RT) void radix_place_kernel(const int* __restrict__
     if (ok && r == 0) at[w][d] = p + __popcll(same);
     __builtin_amdgcn_wave_barrier();
     if (ok) {
-      dst[p] = k;
-      pdst[p] = FIRST ? i : psrc[i];
+      dst[p] = k[u];
+      pdst[p] = v[u];
     }
   }
 }
@@ -166,16 +204,6 @@ __device__ __forceinline__ void store8(float* p, const float (&f)[8]) {
   *(f32x4*)p = f32x4{f[0], f[1], f[2], f[3]};
   *(f32x4*)(p + 4) = f32x4{f[4], f[5], f[6], f[7]};
 }
-// first place of `keys` (sorted, n items, from lo) whose key is >= k
-__device__ __forceinline__ int lower(const int* keys, int lo, int n, int k) {
-  int hi = n;
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (keys[mid] < k) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
-}
 template <bool ACC>
 __device__ __forceinline__ void put_row(float* d, float (&a)[8], float scale) {
   if (ACC) {
@@ -190,41 +218,63 @@ __device__ __forceinline__ void put_row(float* d, float (&a)[8], float scale) {
   store8(d, a);
 }
 
+// first place of `keys` whose key is >= k, by one wave: 64 probes a round
+__device__ __forceinline__ int lower_wave(const int* keys, int n, int k) {
+  const int l = threadIdx.x & 63;
+  int lo = 0, hi = n;  // the answer is in [lo, hi]
+  while (hi - lo > 0) {
+    const int step = (hi - lo + 63) / 64, at = lo + l * step;
+    const unsigned long long m = __ballot(at < hi && keys[min(at, n - 1)] < k);  // a prefix of the lanes
+    const int c = __popcll(m);
+    if (c == 0) return lo;
+    const int nlo = lo + (c - 1) * step + 1;
+    hi = min(hi, lo + c * step);
+    lo = nlo;
+  }
+  return lo;
+}
+
 // lpc lanes share a chunk (8 columns each, `slabs` groups across a row); blocks from `sumb` on zero
-// the rows without tokens, 64 rows a block
+// the rows without tokens, 64 rows a block. A group loads BATCH rows at once, then adds them in order:
+// one row's latency at a time was most of a short batch's 18 us.
+constexpr int BATCH = 8;
 template <typename T, bool ACC>
 __global__ __launch_bounds__(NT) void emb_sum_kernel(const int* __restrict__ keys, const int* __restrict__ perm, int n,
                                                      int V, int W, const T* __restrict__ dy, long long ldy,
                                                      float* __restrict__ dword, float* __restrict__ part, float scale,
-                                                     int lpc, int slabs, int sumb) {
+                                                     int chunk_len, int lpc, int slabs, int sumb) {
   if ((int)blockIdx.x >= sumb) {
-    __shared__ unsigned long long has;
+    __shared__ unsigned has[2];
+    __shared__ int range[2];
     const int r0 = ((int)blockIdx.x - sumb) * 64, nr = min(64, V - r0);
-    if (threadIdx.x < 64) {
-      const int r = r0 + (int)threadIdx.x;
-      bool found = false;
-      if (r < V) {
-        const int p = lower(keys, 0, n, r);
-        found = p < n && keys[p] == r;
-      }
-      const unsigned long long m = __ballot(found);
-      if (threadIdx.x == 0) has = m;
+    if (threadIdx.x < 2) has[threadIdx.x] = 0;
+    if (threadIdx.x < 128) {
+      const int w = threadIdx.x >> 6, p = lower_wave(keys, n, r0 + w * 64);
+      if ((threadIdx.x & 63) == 0) range[w] = p;
     }
     __syncthreads();
-    const unsigned long long m = has;
+    for (int p = range[0] + threadIdx.x; p < range[1]; p += NT) {
+      const int r = keys[p] - r0;
+      if (p == range[0] || keys[p - 1] != keys[p]) atomicOr(&has[r >> 5], 1u << (r & 31));
+    }
+    __syncthreads();
+    const unsigned m0 = has[0], m1 = has[1];
     const int vpr = W >> 2;
-    for (int r = 0; r < nr; ++r) {
-      if ((m >> r) & 1) continue;
-      float* d = dword + (long long)(r0 + r) * W;
-      for (int c = threadIdx.x; c < vpr; c += NT) *(f32x4*)(d + 4 * c) = f32x4{0.f, 0.f, 0.f, 0.f};
+    int r = 0, c = threadIdx.x;
+    float* d = dword + (long long)r0 * W;
+    while (c >= vpr) { c -= vpr; ++r; }
+    for (; r < nr;) {
+      if (!(((r < 32 ? m0 : m1) >> (r & 31)) & 1)) *(f32x4*)(d + (long long)r * W + 4 * c) = f32x4{0.f, 0.f, 0.f, 0.f};
+      c += NT;
+      while (c >= vpr) { c -= vpr; ++r; }
     }
     return;
   }
-  const long long gid = (long long)blockIdx.x * NT + threadIdx.x, unit = gid / lpc;
+  const unsigned gid = blockIdx.x * NT + threadIdx.x, unit = gid / lpc;
   const int chunk = (int)(unit / slabs), col = ((int)(unit % slabs) * lpc + (int)(gid % lpc)) * 8;
-  const int c0 = chunk * CHUNK;
+  const int c0 = chunk * chunk_len;
   if (c0 >= n || col >= W) return;
-  const int c1 = min(n, c0 + CHUNK);
+  const int c1 = min(n, c0 + chunk_len);
   int cur = keys[c0];
   const bool head = c0 > 0 && keys[c0 - 1] == cur;
   bool first = true;
@@ -232,21 +282,32 @@ __global__ __launch_bounds__(NT) void emb_sum_kernel(const int* __restrict__ key
 #pragma unroll
   for (int e = 0; e < 8; ++e) acc[e] = 0.f;
   float* hp = part + ((long long)chunk * 2) * W + col;
-  for (int p = c0; p < c1; ++p) {
-    const int k = keys[p];
-    if (k != cur) {
-      if (first && head) store8(hp, acc);
-      else put_row<ACC>(dword + (long long)cur * W + col, acc, scale);
-      first = false;
-      cur = k;
+  for (int p0 = c0; p0 < c1; p0 += BATCH) {
+    int k[BATCH], t[BATCH];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+    for (int u = 0; u < BATCH; ++u) {
+      k[u] = p0 + u < c1 ? keys[p0 + u] : V;
+      t[u] = perm[min(p0 + u, n - 1)];
     }
-    if (k >= V) return;  // only padding from here on
-    float f[8];
-    load8<T>(f, dy + (long long)perm[p] * ldy + col);
+    typedef T T8 __attribute__((ext_vector_type(8)));
+    T8 row[BATCH];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] += f[e];
+    for (int u = 0; u < BATCH; ++u) row[u] = *(const T8*)(dy + t[u] * ldy + col);
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u) {
+      if (p0 + u >= c1) break;
+      if (k[u] != cur) {
+        if (first && head) store8(hp, acc);
+        else put_row<ACC>(dword + (long long)cur * W + col, acc, scale);
+        first = false;
+        cur = k[u];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+      }
+      if (cur >= V) return;  // only padding from here on
+#pragma unroll
+      for (int e = 0; e < 8; ++e) acc[e] += (float)row[u][e];
+    }
   }
   if (first && head) store8(hp, acc);
   else if (c1 < n && keys[c1] == cur) store8(hp + W, acc);
@@ -258,13 +319,13 @@ __global__ __launch_bounds__(NT) void emb_sum_kernel(const int* __restrict__ key
 template <bool ACC>
 __global__ __launch_bounds__(NT) void emb_join_kernel(const int* __restrict__ keys, int n, int V, int W,
                                                       const float* __restrict__ part, float* __restrict__ dword,
-                                                      float scale, int lpc) {
+                                                      float scale, int chunk_len, int lpc) {
   __shared__ float red[NT * 8];
-  const int chunk = blockIdx.x, c0 = chunk * CHUNK, c1 = c0 + CHUNK;
+  const int chunk = blockIdx.x, c0 = chunk * chunk_len, c1 = c0 + chunk_len;
   if (c1 >= n) return;
   const int k = keys[c1 - 1];
   if (k >= V || keys[c1] != k || (c0 > 0 && keys[c0 - 1] == k)) return;
-  const int last = (lower(keys, c1, n, k + 1) - 1) / CHUNK;
+  const int last = (c1 + lower_wave(keys + c1, n - c1, k + 1) - 1) / chunk_len;
   const int groups = NT / lpc, g = threadIdx.x / lpc, li = threadIdx.x % lpc;
   const int col = (blockIdx.y * lpc + li) * 8;
   const int m = last - chunk, per = (m + groups - 1) / groups;
@@ -274,6 +335,7 @@ __global__ __launch_bounds__(NT) void emb_join_kernel(const int* __restrict__ ke
   if (col < W) {
     if (g == 0) load8<float>(acc, part + ((long long)chunk * 2 + 1) * W + col);
     const int b = chunk + 1 + g * per, e1 = min(last + 1, b + per);
+#pragma unroll 8
     for (int c = b; c < e1; ++c) {
       float f[8];
       load8<float>(f, part + ((long long)c * 2) * W + col);
@@ -303,19 +365,21 @@ int lanes_per_chunk(int W) {
   }
   return best;
 }
+// positions of a chunk
+int chunk_of(long long n) { return n <= 4096 ? 8 : 32; }
 template <typename T>
 void emb_sum_launch(const int* keys, const int* perm, int n, int V, int W, const void* dy, long long ldy, float* dword,
                     float* part, float scale, int acc, hipStream_t s) {
-  const int lpc = lanes_per_chunk(W), slabs = (W / 8 + lpc - 1) / lpc;
-  const long long chunks = ((long long)n + CHUNK - 1) / CHUNK;
+  const int lpc = lanes_per_chunk(W), slabs = (W / 8 + lpc - 1) / lpc, cl = chunk_of(n);
+  const long long chunks = ((long long)n + cl - 1) / cl;
   const int sumb = (int)((chunks * slabs * lpc + NT - 1) / NT), zerob = acc ? 0 : (V + 63) / 64;
   if (sumb + zerob == 0) return;
-  if (acc) hipLaunchKernelGGL((emb_sum_kernel<T, true>), dim3(sumb), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, lpc, slabs, sumb);
-  else hipLaunchKernelGGL((emb_sum_kernel<T, false>), dim3(sumb + zerob), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, lpc, slabs, sumb);
+  if (acc) hipLaunchKernelGGL((emb_sum_kernel<T, true>), dim3(sumb), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb);
+  else hipLaunchKernelGGL((emb_sum_kernel<T, false>), dim3(sumb + zerob), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb);
   if (chunks < 2) return;
   const dim3 g((unsigned)(chunks - 1), slabs);
-  if (acc) hipLaunchKernelGGL(emb_join_kernel<true>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, lpc);
-  else hipLaunchKernelGGL(emb_join_kernel<false>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, lpc);
+  if (acc) hipLaunchKernelGGL(emb_join_kernel<true>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);
+  else hipLaunchKernelGGL(emb_join_kernel<false>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);
 }
 constexpr int COUNT_MAX = 16384;
 }  // namespace
@@ -330,7 +394,7 @@ long long tfk_token_order_scratch(long long T) {
 int tfk_token_order(const int* ids, int T, int V, int* perm, int* keys, int* scratch, hipStream_t s) {
   if (T <= 0) return 0;
   if (T <= COUNT_MAX) {
-    hipLaunchKernelGGL(order_count_kernel, dim3((T + 63) / 64), dim3(1024), 0, s, ids, T, V, perm, keys);
+    hipLaunchKernelGGL(order_count_kernel, dim3((T + OP - 1) / OP), dim3(1024), 0, s, ids, T, V, perm, keys);
     return hipGetLastError() == hipSuccess ? 0 : -1;
   }
   int total = 1;
@@ -356,7 +420,7 @@ int tfk_token_order(const int* ids, int T, int V, int* perm, int* keys, int* scr
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
 // f32 words of workspace that tfk_emb_sorted needs
-long long tfk_emb_sorted_part(long long T, int W) { return (T + CHUNK - 1) / CHUNK * 2 * W; }
+long long tfk_emb_sorted_part(long long T, int W) { return (T + chunk_of(T) - 1) / chunk_of(T) * 2 * W; }
 // dtype: 0 bf16, 1 f16, 2 f32; W % 8 == 0, rows of dy and dword 16-B aligned
 int tfk_emb_sorted(const int* keys, const int* perm, int T, int V, int W, const void* dy, int dtype, long long ldy,
                    float* dword, float* part, float scale, int acc, hipStream_t s) {

@@ -110,11 +110,93 @@ __device__ __forceinline__ void load_vec(Vec<T>& v, const T* x, int i, int V) {
   }
 }
 
-template <typename T>
+// The k best of a part. Each wave finds the k-th largest of its 64 lane maxima by bisection over the bits of
+// the ordered value; the largest of these over the block bounds the part's k-th best from below, so the
+// few logits that are not below it hold the answer. They are listed in LDS and ranked by counting the
+// larger keys. Where the list overflows (hundreds of equal logits) k rounds of a block maximum decide,
+// over the part read again (its registers would cost every call occupancy: 152 VGPRs instead of 93).
+constexpr int CAND = 1024;
+struct TopShared {
+  u64 key[CAND];
+  u64 wkey[2][NW];
+  float bound[NW];
+  int n;
+};
+template <typename T, typename Put>
+__device__ __forceinline__ void top_k(const Vec<T> (&v)[NV], const T* x, int V, int v0, int v1, float lane_max, int k,
+                                      TopShared& sh, Put put) {
+  constexpr int N = Vec<T>::N;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int lim = min(V, v1 * N);
+  const unsigned om = v0 + (int)threadIdx.x < v1 ? (unsigned)(order_key(lane_max, 0) >> 32) : 0u;
+  unsigned t = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const unsigned c = t | (1u << bit);
+    if (__popcll(__ballot(om >= c)) >= k) t = c;
+  }
+  if (l == 0) sh.bound[w] = t == 0 ? -INFINITY : key_val((u64)t << 32);
+  if (threadIdx.x == 0) sh.n = 0;
+  __syncthreads();
+  float bound = sh.bound[0];
+#pragma unroll
+  for (int u = 1; u < NW; ++u) bound = fmaxf(bound, sh.bound[u]);
+#pragma unroll
+  for (int c = 0; c < NV; ++c) {
+    float m = v[c].at(0);
+#pragma unroll
+    for (int e = 1; e < N; ++e) m = fmaxf(m, v[c].at(e));
+    // !(x < bound): NaN counts as largest (a vector of NaN only has m = NaN)
+    if (!(m < bound) || m != m) {
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int col = (v0 + c * NT + (int)threadIdx.x) * N + e;
+        if (!(v[c].at(e) < bound) && col < lim) {
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < CAND) sh.key[at] = order_key(v[c].at(e), col);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  const int n = sh.n;
+  if (n <= CAND) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const u64 key = sh.key[i];
+      int r = 0;
+      for (int j = 0; j < n; ++j) r += sh.key[j] > key ? 1 : 0;
+      if (r < k) put(r, key);
+    }
+    for (int j = n + (int)threadIdx.x; j < k; j += NT) put(j, 0ull);  // a part shorter than k
+    return;
+  }
+  u64 prev = ~0ull;
+  for (int j = 0; j < k; ++j) {
+    u64 best = 0;
+    for (int i = v0 + (int)threadIdx.x; i < v1; i += NT) {
+      Vec<T> y;
+      load_vec<T>(y, x, i, V);
+#pragma unroll
+      for (int e = 0; e < N; ++e) {
+        const int col = i * N + e;
+        const u64 key = col < lim ? order_key(y.at(e), col) : 0;
+        best = key < prev && key > best ? key : best;
+      }
+    }
+    best = wave_max64(best);
+    if (l == 0) sh.wkey[j & 1][w] = best;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < NW; ++u) best = sh.wkey[j & 1][u] > best ? sh.wkey[j & 1][u] : best;
+    prev = best;
+    if (threadIdx.x == 0) put(j, best);
+  }
+}
+
+template <typename T, bool TOP>
 __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(FwdParams p) {
   constexpr int N = Vec<T>::N;
   __shared__ Stat wst[NW];
-  __shared__ u64 wkey[2][NW];
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const T* x = (const T*)p.x + (long long)row * p.ld;
@@ -159,50 +241,43 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(FwdParams p) {
     if (p.parts == 1) write_row<T>(p, row, st);
     else p.pstat[(long long)row * p.parts + part] = st;
   }
-  if (p.k == 0) return;
-  const float ls = st.s == 0.f ? 0.f : logf(st.s);
-  // the k best, one after another: each round takes the largest key below the last one
-  u64 prev = ~0ull;
-  for (int j = 0; j < p.k; ++j) {
-    u64 best = 0;
-#pragma unroll
-    for (int c = 0; c < NV; ++c)
-#pragma unroll
-      for (int e = 0; e < N; ++e) {
-        const int col = (v0 + c * NT + (int)threadIdx.x) * N + e;
-        const u64 key = col < min(p.V, v1 * N) ? order_key(v[c].at(e), col) : 0;
-        best = key < prev && key > best ? key : best;
-      }
-    best = wave_max64(best);
-    if (l == 0) wkey[j & 1][w] = best;
-    __syncthreads();
-#pragma unroll
-    for (int u = 0; u < NW; ++u) best = wkey[j & 1][u] > best ? wkey[j & 1][u] : best;
-    prev = best;
-    if (threadIdx.x == 0) {
-      if (p.parts == 1) write_top(p, row, j, best, st, ls);
-      else p.pkeys[((long long)row * p.parts + part) * p.k + j] = best;
-    }
+  if constexpr (TOP) {
+    __shared__ TopShared sh;
+    const float ls = st.s == 0.f ? 0.f : logf(st.s);
+    top_k<T>(v, x, p.V, v0, v1, m, p.k, sh, [&](int j, u64 key) {
+      if (p.parts == 1) write_top(p, row, j, key, st, ls);
+      else p.pkeys[((long long)row * p.parts + part) * p.k + j] = key;
+    });
   }
 }
 
 // one block per row: joins its parts; the k best of parts * k candidates by counting the larger ones
-template <typename T>
-__global__ __launch_bounds__(64) void logprobs_join_kernel(FwdParams p) {
+constexpr int JT = 1024;  // candidates staged at a time
+template <typename T, bool TOP>
+__global__ __launch_bounds__(TOP ? NT : 64) void logprobs_join_kernel(FwdParams p) {
   const int row = blockIdx.x;
   const Stat* ps = p.pstat + (long long)row * p.parts;
   Stat st = ps[0];
   for (int u = 1; u < p.parts; ++u) st = join(st, ps[u]);
   if (threadIdx.x == 0) write_row<T>(p, row, st);
-  if (p.k == 0) return;
-  const float ls = st.s == 0.f ? 0.f : logf(st.s);
-  const u64* pk = p.pkeys + (long long)row * p.parts * p.k;
-  const int n = p.parts * p.k;
-  for (int i = threadIdx.x; i < n; i += 64) {
-    const u64 key = pk[i];
-    int r = 0;
-    for (int j = 0; j < n; ++j) r += pk[j] > key ? 1 : 0;
-    if (key != 0 && r < p.k) write_top(p, row, r, key, st, ls);
+  if constexpr (TOP) {
+    __shared__ u64 keys[JT];
+    const float ls = st.s == 0.f ? 0.f : logf(st.s);
+    const int n = p.parts * p.k;
+    const u64* pk = p.pkeys + (long long)row * n;
+    for (int i0 = 0; i0 < n; i0 += NT) {
+      const int i = i0 + (int)threadIdx.x;
+      const u64 key = i < n ? pk[i] : 0;
+      int r = 0;
+      for (int j0 = 0; j0 < n; j0 += JT) {
+        const int m = min(JT, n - j0);
+        __syncthreads();
+        for (int j = threadIdx.x; j < m; j += NT) keys[j] = pk[j0 + j];
+        __syncthreads();
+        for (int j = 0; j < m; ++j) r += keys[j] > key ? 1 : 0;
+      }
+      if (key != 0 && r < p.k) write_top(p, row, r, key, st, ls);
+    }
   }
 }
 
@@ -293,9 +368,11 @@ int tfk_logprobs_fwd(const void* x, int dtype, const int* ids, int T, int V, lon
   p.pkeys = (u64*)ws;
   p.pstat = (Stat*)((u64*)ws + (long long)T * p.parts * k);
   const dim3 g((unsigned)((long long)T * p.parts));
-#define TFK_LP(T_)                                                                       \
-  hipLaunchKernelGGL(logprobs_fwd_kernel<T_>, g, dim3(NT), 0, s, p);                      \
-  if (p.parts > 1) hipLaunchKernelGGL(logprobs_join_kernel<T_>, dim3(T), dim3(64), 0, s, p);
+#define TFK_LP(T_)                                                                                              \
+  if (k) hipLaunchKernelGGL((logprobs_fwd_kernel<T_, true>), g, dim3(NT), 0, s, p);                             \
+  else hipLaunchKernelGGL((logprobs_fwd_kernel<T_, false>), g, dim3(NT), 0, s, p);                              \
+  if (p.parts > 1 && k) hipLaunchKernelGGL((logprobs_join_kernel<T_, true>), dim3(T), dim3(NT), 0, s, p);       \
+  else if (p.parts > 1) hipLaunchKernelGGL((logprobs_join_kernel<T_, false>), dim3(T), dim3(64), 0, s, p);
   if (dtype == 0) { TFK_LP(bf16) } else if (dtype == 1) { TFK_LP(f16) } else { TFK_LP(float) }
 #undef TFK_LP
   return hipGetLastError() == hipSuccess ? 0 : -1;
