@@ -13,7 +13,8 @@
 extern "C" {
 int tfk_shaped_fwd(const void*, const void*, const void*, void*, float*, int, const long long*, const long long*,
                    const int*, const int*, const int*, const int*, const float*, float, float, int, float,
-                   unsigned long long, hipStream_t);
+                   unsigned long long, float*, hipStream_t);
+long long tfk_shaped_fwd_ws(const long long*, float);
 int tfk_shaped_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*,
                    void*, int, const long long*, const long long*, const long long*, const int*, const int*, const int*,
                    const int*, const float*, float, float, int, float, unsigned long long, hipStream_t);
@@ -74,8 +75,8 @@ void check_cols(const torch::Tensor& t, const torch::Tensor& ref, long long off,
   if (write)
     TORCH_CHECK(B == 1 || bs >= (S - 1) * rs + W || (bs >= W && rs >= (B - 1) * bs + W), n, ": tokens overlap");
 }
-void check_shape(const std::vector<int64_t>& s, const std::vector<int64_t>& st, double scale, double cap, double p_drop) {
-  TORCH_CHECK(s.size() == 6 && st.size() == 8, "attention shape [B,H,Hk,Sq,Sk,D], strides [q,k,v,o: batch, token]");
+void check_shape(const std::vector<int64_t>& s, double scale, double cap, double p_drop) {
+  TORCH_CHECK(s.size() == 6, "attention shape [B,H,Hk,Sq,Sk,D]");
   for (auto v : s) TORCH_CHECK(v >= 1 && v <= 0x7fffffff, "bad attention shape");
   TORCH_CHECK(s[1] % s[2] == 0, "heads must be a multiple of key heads");
   TORCH_CHECK(s[5] == 64 || s[5] == 128, "head dim must be 64 or 128, got ", s[5]);
@@ -102,66 +103,89 @@ Masks masks(const Opt& kv_len, const Opt& q_start, const Opt& prefix, const Opt&
                opt_ptr<const int>(docs), opt_ptr<const float>(slopes)};
 }
 
-void shaped_fwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch::Tensor v, int64_t vo, torch::Tensor out,
-                torch::Tensor lse, std::vector<int64_t> shape, std::vector<int64_t> strides, Opt kv_len, Opt q_start,
-                Opt prefix, Opt docs, Opt slopes, double scale, double cap, bool causal, double p_drop, int64_t seed) {
-  const int f16 = type_code(q, false, "q");
-  const c10::DeviceGuard guard(q.device());
-  check_shape(shape, strides, scale, cap, p_drop);
+// [batch, token] strides of a 2-D [B * S, width] or 3-D [B, S', width] buffer
+void buf_strides(const torch::Tensor& t, long long S, long long* st, const char* n) {
+  TORCH_CHECK(t.dim() == 2 || t.dim() == 3, n, " must be [B*S, width] or [B, S', width]");
+  st[1] = t.stride(-2);
+  st[0] = t.dim() == 3 ? t.stride(0) : S * st[1];
+}
+struct Call {
+  int f16;
+  long long sh[6], st[8];
+};
+// shape [B, H, Hk, Sq, Sk, D]; fills everything but the output's strides
+Call check_call(const torch::Tensor& q, int64_t qo, const torch::Tensor& k, int64_t ko, const torch::Tensor& v, int64_t vo,
+                const std::vector<int64_t>& shape, double scale, double cap, double p_drop) {
+  Call c;
+  c.f16 = type_code(q, false, "q");
+  check_shape(shape, scale, cap, p_drop);
+  for (int i = 0; i < 6; ++i) c.sh[i] = shape[i];
   const long long B = shape[0], H = shape[1], Hk = shape[2], Sq = shape[3], Sk = shape[4], D = shape[5];
-  check_cols(q, q, qo, strides[0], strides[1], B, Sq, H * D, false, "q");
-  check_cols(k, q, ko, strides[2], strides[3], B, Sk, Hk * D, false, "k");
-  check_cols(v, q, vo, strides[4], strides[5], B, Sk, Hk * D, false, "v");
-  check_cols(out, q, 0, strides[6], strides[7], B, Sq, H * D, true, "out");
-  need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
+  buf_strides(q, Sq, c.st, "q");
+  buf_strides(k, Sk, c.st + 2, "k");
+  buf_strides(v, Sk, c.st + 4, "v");
+  c.st[6] = Sq * H * D;
+  c.st[7] = H * D;
+  check_cols(q, q, qo, c.st[0], c.st[1], B, Sq, H * D, false, "q");
+  check_cols(k, q, ko, c.st[2], c.st[3], B, Sk, Hk * D, false, "k");
+  check_cols(v, q, vo, c.st[4], c.st[5], B, Sk, Hk * D, false, "v");
+  return c;
+}
+void* at(const torch::Tensor& t, int64_t o) { return (void*)((char*)t.data_ptr() + 2 * o); }
+
+std::tuple<torch::Tensor, torch::Tensor> shaped_fwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch::Tensor v,
+                                                    int64_t vo, std::vector<int64_t> shape, Opt kv_len, Opt q_start,
+                                                    Opt prefix, Opt docs, Opt slopes, double scale, double cap, bool causal,
+                                                    double p_drop, int64_t seed) {
+  const Call c = check_call(q, qo, k, ko, v, vo, shape, scale, cap, p_drop);
+  const c10::DeviceGuard guard(q.device());
   const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
-  std::vector<long long> sh(shape.begin(), shape.end()), st(strides.begin(), strides.end());
-  auto at = [](torch::Tensor& t, int64_t o) { return (void*)((char*)t.data_ptr() + 2 * o); };
-  check_rc(tfk_shaped_fwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), lse.data_ptr<float>(), f16, sh.data(), st.data(),
+  torch::Tensor out = at::empty({c.sh[0] * c.sh[3], c.sh[1] * c.sh[5]}, q.options());
+  torch::Tensor lse = at::empty({c.sh[0], c.sh[1], c.sh[3]}, q.options().dtype(at::kFloat)), ws;
+  const long long wn = tfk_shaped_fwd_ws(c.sh, (float)p_drop);
+  if (wn) ws = at::empty({wn}, lse.options());
+  check_rc(tfk_shaped_fwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), lse.data_ptr<float>(), c.f16, c.sh, c.st,
                           m.kv_len, m.q_start, m.prefix, m.docs, m.slopes, (float)scale, (float)cap, causal ? 1 : 0,
-                          (float)p_drop, (unsigned long long)seed, stream_of(q)),
+                          (float)p_drop, (unsigned long long)seed, wn ? ws.data_ptr<float>() : nullptr, stream_of(q)),
            "shaped_fwd");
+  return {out, lse};
 }
 
 void shaped_bwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch::Tensor v, int64_t vo, torch::Tensor out,
                 torch::Tensor dout, torch::Tensor lse, torch::Tensor dq, int64_t dqo, torch::Tensor dk, int64_t dko,
-                torch::Tensor dv, int64_t dvo, std::vector<int64_t> shape, std::vector<int64_t> strides,
-                std::vector<int64_t> gstrides, Opt kv_len, Opt q_start, Opt prefix, Opt docs, Opt slopes, double scale,
-                double cap, bool causal, double p_drop, int64_t seed) {
-  const int f16 = type_code(q, false, "q");
+                torch::Tensor dv, int64_t dvo, std::vector<int64_t> shape, Opt kv_len, Opt q_start, Opt prefix, Opt docs,
+                Opt slopes, double scale, double cap, bool causal, double p_drop, int64_t seed) {
+  const Call c = check_call(q, qo, k, ko, v, vo, shape, scale, cap, p_drop);
   const c10::DeviceGuard guard(q.device());
-  check_shape(shape, strides, scale, cap, p_drop);
-  TORCH_CHECK(gstrides.size() == 6, "gstrides [dq,dk,dv: batch, token]");
   const long long B = shape[0], H = shape[1], Hk = shape[2], Sq = shape[3], Sk = shape[4], D = shape[5];
-  check_cols(q, q, qo, strides[0], strides[1], B, Sq, H * D, false, "q");
-  check_cols(k, q, ko, strides[2], strides[3], B, Sk, Hk * D, false, "k");
-  check_cols(v, q, vo, strides[4], strides[5], B, Sk, Hk * D, false, "v");
-  check_cols(out, q, 0, strides[6], strides[7], B, Sq, H * D, false, "out");
-  check_cols(dout, q, 0, strides[6], strides[7], B, Sq, H * D, false, "dout");
-  check_cols(dq, q, dqo, gstrides[0], gstrides[1], B, Sq, H * D, true, "dq");
-  check_cols(dk, q, dko, gstrides[2], gstrides[3], B, Sk, Hk * D, true, "dk");
-  check_cols(dv, q, dvo, gstrides[4], gstrides[5], B, Sk, Hk * D, true, "dv");
+  long long gs[6];
+  buf_strides(dq, Sq, gs, "dq");
+  buf_strides(dk, Sk, gs + 2, "dk");
+  buf_strides(dv, Sk, gs + 4, "dv");
+  TORCH_CHECK(out.is_contiguous() && dout.is_contiguous(), "out and dout must be contiguous [B*Sq, H*D]");
+  check_cols(out, q, 0, c.st[6], c.st[7], B, Sq, H * D, false, "out");
+  check_cols(dout, q, 0, c.st[6], c.st[7], B, Sq, H * D, false, "dout");
+  check_cols(dq, q, dqo, gs[0], gs[1], B, Sq, H * D, true, "dq");
+  check_cols(dk, q, dko, gs[2], gs[3], B, Sk, Hk * D, true, "dk");
+  check_cols(dv, q, dvo, gs[4], gs[5], B, Sk, Hk * D, true, "dv");
   need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
   const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
-  torch::Tensor delta = torch::empty({B * H * Sq}, lse.options());
-  std::vector<long long> sh(shape.begin(), shape.end()), st(strides.begin(), strides.end()),
-      gs(gstrides.begin(), gstrides.end());
-  auto at = [](torch::Tensor& t, int64_t o) { return (void*)((char*)t.data_ptr() + 2 * o); };
+  torch::Tensor delta = at::empty({B * H * Sq}, lse.options());
   check_rc(tfk_shaped_bwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
-                          delta.data_ptr<float>(), at(dq, dqo), at(dk, dko), at(dv, dvo), f16, sh.data(), st.data(),
-                          gs.data(), m.kv_len, m.q_start, m.prefix, m.docs, m.slopes, (float)scale, (float)cap,
-                          causal ? 1 : 0, (float)p_drop, (unsigned long long)seed, stream_of(q)),
+                          delta.data_ptr<float>(), at(dq, dqo), at(dk, dko), at(dv, dvo), c.f16, c.sh, c.st, gs, m.kv_len,
+                          m.q_start, m.prefix, m.docs, m.slopes, (float)scale, (float)cap, causal ? 1 : 0, (float)p_drop,
+                          (unsigned long long)seed, stream_of(q)),
            "shaped_bwd");
 }
 
-void doc_spans(torch::Tensor ids, torch::Tensor out) {
+torch::Tensor doc_spans(torch::Tensor ids) {
   need(ids, at::kInt, "ids");
   TORCH_CHECK(ids.dim() == 2 && ids.size(1) <= 0x3fffffff, "ids must be [B, S]");
-  need_vec(out, at::kInt, 2 * ids.numel(), ids, "out");
-  need_aligned(out, 8, "out");
   const c10::DeviceGuard guard(ids.device());
+  torch::Tensor out = at::empty({ids.size(0), ids.size(1), 2}, ids.options());
   check_rc(tfk_doc_spans(ids.data_ptr<int>(), ids.size(0), (int)ids.size(1), out.data_ptr<int>(), stream_of(ids)),
            "doc_spans");
+  return out;
 }
 
 // logits [T, cols] (unit column stride), the first V columns are classes
@@ -175,25 +199,30 @@ int check_logits(const torch::Tensor& x, const torch::Tensor& ids, int64_t V, in
   need_vec(ids, at::kInt, x.size(0), x, "ids");
   return dt;
 }
-void logprobs_fwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_t k, int64_t ignore, torch::Tensor logp,
-                  torch::Tensor ent, torch::Tensor lse, torch::Tensor norm, Opt top_logp, Opt top_ids) {
+// -> logp, entropy, lse [T], norm [T, 2], top_logp, top_ids [T, k] (None for k = 0)
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, Opt, Opt> logprobs_fwd(torch::Tensor x,
+                                                                                             torch::Tensor ids, int64_t V,
+                                                                                             int64_t k, int64_t ignore) {
   const int dt = check_logits(x, ids, V, k);
   const c10::DeviceGuard guard(x.device());
   const long long T = x.size(0);
-  need_vec(logp, at::kFloat, T, x, "logp"); need_vec(ent, at::kFloat, T, x, "entropy"); need_vec(lse, at::kFloat, T, x, "lse");
-  need_vec(norm, at::kFloat, 2 * T, x, "norm");
-  TORCH_CHECK(k == 0 || (top_logp.has_value() && top_ids.has_value()), "top_k needs its outputs");
-  need_opt(top_logp, at::kFloat, T * k, x, "top_logp");
-  need_opt(top_ids, at::kInt, T * k, x, "top_ids");
+  const auto f = x.options().dtype(at::kFloat);
+  torch::Tensor logp = at::empty({T}, f), ent = at::empty({T}, f), lse = at::empty({T}, f), norm = at::empty({T, 2}, f), w;
+  Opt tl, ti;
+  if (k) {
+    tl = at::empty({T, k}, f);
+    ti = at::empty({T, k}, ids.options());
+  }
   const long long ws = tfk_logprobs_ws(T, (int)V, dt, (int)k);
-  torch::Tensor w = torch::empty({ws}, x.options().dtype(at::kByte));
+  if (ws) w = at::empty({ws}, x.options().dtype(at::kByte));
   check_rc(tfk_logprobs_fwd(x.data_ptr(), dt, ids.data_ptr<int>(), (int)T, (int)V, x.stride(0), (int)k, (int)ignore,
                             logp.data_ptr<float>(), ent.data_ptr<float>(), lse.data_ptr<float>(), norm.data_ptr<float>(),
-                            opt_ptr<float>(top_logp), opt_ptr<int>(top_ids), w.data_ptr(), stream_of(x)),
+                            opt_ptr<float>(tl), opt_ptr<int>(ti), ws ? w.data_ptr() : nullptr, stream_of(x)),
            "logprobs_fwd");
+  return {logp, ent, lse, norm, tl, ti};
 }
-void logprobs_bwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_t ignore, torch::Tensor norm, torch::Tensor ent,
-                  Opt top_ids, Opt dlogp, Opt dent, Opt dtop, torch::Tensor dx) {
+torch::Tensor logprobs_bwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_t ignore, torch::Tensor norm,
+                           torch::Tensor ent, Opt top_ids, Opt dlogp, Opt dent, Opt dtop) {
   const bool top = dtop.has_value() && dtop->defined();
   TORCH_CHECK(!top || (top_ids.has_value() && top_ids->defined() && dtop->dim() == 2), "dtop [T, k] needs top_ids");
   const int64_t k = top ? dtop->size(1) : 0;
@@ -203,24 +232,27 @@ void logprobs_bwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_t ignore,
   need_vec(norm, at::kFloat, 2 * T, x, "norm"); need_vec(ent, at::kFloat, T, x, "entropy");
   need_opt(dlogp, at::kFloat, T, x, "dlogp"); need_opt(dent, at::kFloat, T, x, "dentropy");
   if (top) { need_opt(dtop, at::kFloat, T * k, x, "dtop"); need_opt(top_ids, at::kInt, T * k, x, "top_ids"); }
-  need_vec(dx, x.scalar_type(), T * x.size(1), x, "dlogits");
+  torch::Tensor dx = at::empty({T, x.size(1)}, x.options());
   check_rc(tfk_logprobs_bwd(x.data_ptr(), dt, ids.data_ptr<int>(), (int)T, (int)V, x.stride(0), (int)k, (int)ignore,
                             norm.data_ptr<float>(), ent.data_ptr<float>(), top ? opt_ptr<const int>(top_ids) : nullptr,
                             opt_ptr<const float>(dlogp), opt_ptr<const float>(dent), top ? opt_ptr<const float>(dtop) : nullptr,
                             dx.data_ptr(), x.size(1), (int)x.size(1), stream_of(x)),
            "logprobs_bwd");
+  return dx;
 }
 
-void token_order(torch::Tensor ids, int64_t V, torch::Tensor perm, torch::Tensor keys) {
+std::tuple<torch::Tensor, torch::Tensor> token_order(torch::Tensor ids, int64_t V) {
   need(ids, at::kInt, "ids");
   const long long T = ids.numel();
   TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 0x3fffffff, "token_order: V ", V, ", tokens ", T);
-  need_vec(perm, at::kInt, T, ids, "perm"); need_vec(keys, at::kInt, T, ids, "keys");
   const c10::DeviceGuard guard(ids.device());
-  torch::Tensor w = torch::empty({tfk_token_order_scratch(T)}, ids.options());
+  torch::Tensor perm = at::empty({T}, ids.options()), keys = at::empty({T}, ids.options()), w;
+  const long long ws = tfk_token_order_scratch(T);
+  if (ws) w = at::empty({ws}, ids.options());
   check_rc(tfk_token_order(ids.data_ptr<int>(), (int)T, (int)V, perm.data_ptr<int>(), keys.data_ptr<int>(),
-                           w.data_ptr<int>(), stream_of(ids)),
+                           ws ? w.data_ptr<int>() : nullptr, stream_of(ids)),
            "token_order");
+  return {perm, keys};
 }
 void embedding_bwd_sorted(torch::Tensor perm, torch::Tensor keys, torch::Tensor dy, torch::Tensor dword, double scale,
                           bool accumulate) {
@@ -238,7 +270,7 @@ void embedding_bwd_sorted(torch::Tensor perm, torch::Tensor keys, torch::Tensor 
   need_aligned(dy, 16, "dy"); need_aligned(dword, 16, "dword");
   need_vec(perm, at::kInt, T, dy, "order"); need_vec(keys, at::kInt, T, dy, "order");
   const c10::DeviceGuard guard(dy.device());
-  torch::Tensor part = torch::empty({tfk_emb_sorted_part(T, (int)W)}, dword.options());
+  torch::Tensor part = at::empty({tfk_emb_sorted_part(T, (int)W)}, dword.options());
   check_rc(tfk_emb_sorted(keys.data_ptr<int>(), perm.data_ptr<int>(), (int)T, (int)V, (int)W, dy.data_ptr(), dt,
                           dy.stride(0), dword.data_ptr<float>(), part.data_ptr<float>(), (float)scale, accumulate ? 1 : 0,
                           stream_of(dy)),

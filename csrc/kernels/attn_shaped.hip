@@ -26,6 +26,7 @@
 // is read with the same row order: two ds_read_b64_tr_b16 of rows 4h.. and 8 + 4h.. of each 16.
 // LDS rows are D elements, their 16-byte chunks XOR-swizzled (swz): conflict-free for both reads.
 #include "common.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace {
@@ -83,16 +84,22 @@ __device__ __forceinline__ float pair_max(float v) {  // over lanes l, l ^ 32
   const float a = lane_swap32(v, o);
   return fmaxf(a, o);
 }
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-  return v;
+// wave-wide integer extremes by DPP and permlane swaps (common.h wave_sum's butterfly)
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, false);
 }
 __device__ __forceinline__ int wave_max_i(int v) {
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
-  return v;
+  v = max(v, dpp_i<0xB1>(v));
+  v = max(v, dpp_i<0x4E>(v));
+  v = max(v, dpp_i<0x141>(v));
+  v = max(v, dpp_i<0x140>(v));
+  auto a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  v = max((int)a[0], (int)a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane(max((int)b[0], (int)b[1]));
 }
+__device__ __forceinline__ int wave_min_i(int v) { return ~wave_max_i(~v); }
 // LDS-only block barrier: the next tile's global loads stay in flight across it
 __device__ __forceinline__ void lds_bar() {
   asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -789,6 +796,236 @@ __global__ __launch_bounds__(NW * 64, D == 128 ? 1 : 2) void shaped_dkv_kernel(S
   }
 }
 
+// ------------------------------------------------------------------------------- few query rows
+// The forward for at most 32 rows (queries x heads of a group): serving's single tokens. All waves of a
+// block hold the same rows and divide the keys (8 KiB of K at a time), so the work along the cache is split
+// NW ways inside a block and `splits` ways over blocks; each block takes an even share of the keys
+// that its rows see (the lengths are device data). Bound by reading K and V once: K goes from memory
+// straight into operand registers, V through the wave's own LDS (no block barrier in the loop). The
+// waves' (m, l, O) meet in LDS, those of the blocks in shaped_few_join_kernel.
+constexpr int FW = 8;  // waves
+template <typename T, int D>
+__global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int splits, float* __restrict__ part) {
+  constexpr int KB = 128 / D, KEYS = 32 * KB;  // a wave's tile: 8 KiB of K, of V
+  constexpr int VB = KEYS * D * 2;             // (the f32 accumulators take D / 64 * VB)
+  __shared__ __attribute__((aligned(16))) char smem[FW * VB];
+  __shared__ float ml[2][FW][32];
+  const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5, r = l & 31;
+  Offs<D> fo;
+  fo.init();
+  const int inst = blockIdx.x / splits, split = blockIdx.x % splits;
+  const int b = inst / p.Hk, hk = inst % p.Hk, R = p.G * p.Sq;
+  const bool valid = r < R;
+  const int g = valid ? r / p.Sq : 0, q = valid ? r % p.Sq : 0, head = hk * p.G + g;
+  const int shift = q_shift(p, b), kvl = min(p.kv_len ? p.kv_len[b] : p.Sk, p.Sk);
+  Span sp = valid ? span_of(p, b, q, shift, kvl) : Span{0, 0};
+  const bool sees = sp.hi > sp.lo;
+  const int ulo = wave_min_i(sees ? sp.lo : 0x7fffffff), uhi = wave_max_i(sees ? sp.hi : 0);
+  const int ilo = wave_max_i(sees ? sp.lo : 0), ihi = wave_min_i(sees ? sp.hi : 0x7fffffff);
+  const int a0 = uhi > 0 ? ulo / KEYS : 0, an = (uhi + KEYS - 1) / KEYS - a0, per = (an + splits - 1) / splits;
+  const int t1 = a0 + min(an, (split + 1) * per);
+  int t = a0 + split * per + w;
+
+  const T* Qr = (const T*)p.q + b * p.q_bs + q * p.q_rs + head * D;
+  const T* Kb = (const T*)p.k + b * p.k_bs + hk * D + 8 * h;
+  const T* Vb = (const T*)p.v + b * p.v_bs + hk * D;
+  typename Ty<T>::x8 qf[D / 16];
+#pragma unroll
+  for (int kk = 0; kk < D / 16; ++kk) qf[kk] = frag_mem<T>(Qr, kk, sees);
+  const Score sc(p);
+  const float slope = sc.biased ? p.slopes[head] * LOG2E : 0.f;
+  const int pos = q + shift;
+  float m = -INFINITY, lsum = 0.f;
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
+
+  constexpr int NVV = KEYS * D / 8 / 64;  // 16-byte vectors of V a lane moves
+  char* V_ = smem + w * VB;
+  u32x4 kn[KB][D / 16], vn[NVV];
+  bool vok[NVV];
+  auto load = [&](int tt) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const T* kr = Kb + min(tt * KEYS + kb * 32 + r, p.Sk - 1) * p.k_rs;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) kn[kb][kk] = *(const u32x4*)(kr + kk * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < NVV; ++i) {
+      const int c = l + i * 64, j = tt * KEYS + c / (D / 8), jc = min(j, p.Sk - 1);
+      vn[i] = *(const u32x4*)(Vb + jc * p.v_rs + (c % (D / 8)) * 8);
+      vok[i] = j >= ulo && j < uhi;
+      if (p.docs) {
+        const int2 d = p.docs[(long long)b * p.Sk + jc];
+        vok[i] = vok[i] && d.y > d.x;
+      }
+    }
+  };
+  if (t < t1) load(t);  // (no load past the end: the block barriers behind the loop would wait for it)
+  for (; t < t1; t += FW) {
+    const int k0 = t * KEYS;
+    f32x16 s[KB];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) s[kb] = Ty<T>::mfma(__builtin_bit_cast(typename Ty<T>::x8, kn[kb][kk]), qf[kk], s[kb]);
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < NVV; ++i) {
+      const int c = l + i * 64, row = c / (D / 8);
+      const u32x4 z = u32x4{0u, 0u, 0u, 0u};
+      *(u32x4*)(V_ + row * 2 * D + (((c % (D / 8)) ^ swz<D>(row)) << 4)) = vok[i] ? vn[i] : z;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (t + FW < t1) load(t + FW);
+    if (sc.capped) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] = sc.capl * sc.th(s[kb][e]);
+    }
+    if (sc.biased) {
+      const float sl = sc.capped ? 1.f : p.scale * LOG2E, d0 = (float)(pos - k0 - 4 * h);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[kb][e] = fmaf(-slope, fabsf(d0 - (float)(32 * kb + srow(e))), s[kb][e] * sl);
+    }
+    if (!(k0 >= ilo && k0 + KEYS <= ihi)) {
+      const unsigned base = (unsigned)(k0 + 4 * h - sp.lo), len = (unsigned)(sp.hi - sp.lo);
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (base + (unsigned)(32 * kb + srow(e)) >= len) s[kb][e] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
+    mx = pair_max(mx);
+    const float mnew = fmaxf(m, mx * sc.mult), muse = mnew == -INFINITY ? 0.f : mnew, alpha = ex2(m - muse);
+    float rs = 0.f;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[kb][e] = ex2(fmaf(s[kb][e], sc.mult, -muse));
+        rs += s[kb][e];
+      }
+    lsum = fmaf(lsum, alpha, xor_sum<32>(rs));
+    m = mnew;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
+#pragma unroll
+    for (int kc = 0; kc < 2 * KB; ++kc) {
+      const typename Ty<T>::x8 pf = pack8<T>(s[kc >> 1], kc & 1);
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db) o[db] = Ty<T>::mfma(frag_tr<T, D>(V_, fo, kc, db), pf, o[db]);
+    }
+  }
+  // the waves' parts: a common maximum, then the sums in a tree
+  if (h == 0) { ml[0][w][r] = m; ml[1][w][r] = lsum; }
+  __syncthreads();
+  float M = ml[0][0][r], L = 0.f;
+#pragma unroll
+  for (int u = 1; u < FW; ++u) M = fmaxf(M, ml[0][u][r]);
+  const float Mu = M == -INFINITY ? 0.f : M;
+#pragma unroll
+  for (int u = 0; u < FW; ++u) L = fmaf(ml[1][u][r], ex2(ml[0][u][r] - Mu), L);
+  const float own = ex2(m - Mu);
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[db][e] *= own;
+#pragma unroll
+  for (int half = FW / 2; half > 0; half >>= 1) {  // waves half .. 2 half - 1 hand theirs to w - half
+    f32x4* x = (f32x4*)smem + (w & (half - 1)) * (D / 8) * 64 + l;
+    if (w >= half && w < 2 * half) {
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) x[(db * 4 + e / 4) * 64] = f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]};
+    }
+    __syncthreads();
+    if (w < half) {
+#pragma unroll
+      for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+          const f32x4 y = x[(db * 4 + e / 4) * 64];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) o[db][e + u] += y[u];
+        }
+    }
+    __syncthreads();
+  }
+  if (w != 0 || !valid) return;
+  if (splits > 1) {
+    float* P = part + ((long long)blockIdx.x * R + r) * D + 4 * h;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; e += 4)
+        *(f32x4*)(P + db * 32 + srow(e)) = f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]};
+    if (h == 0) {
+      float* S = part + (long long)gridDim.x * R * D + ((long long)blockIdx.x * R + r) * 2;
+      S[0] = M;
+      S[1] = L;
+    }
+    return;
+  }
+  const float inv = sees && L != 0.f ? 1.f / L : 0.f;
+  T* O = (T*)p.out + b * p.o_bs + q * p.o_rs + head * D + 4 * h;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) {
+      typename Ty<T>::x4 v;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = (T)(sees ? o[db][e + u] * inv : 0.f);
+      *(typename Ty<T>::x4*)(O + db * 32 + srow(e)) = v;
+    }
+  if (h == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = sees && L != 0.f ? (M + __log2f(L)) * LN2 : INFINITY;
+}
+// one wave per (instance, row): the splits' parts in order
+template <typename T, int D>
+__global__ __launch_bounds__(64) void shaped_few_join_kernel(Shaped p, int splits, const float* __restrict__ part) {
+  const int R = p.G * p.Sq, inst = blockIdx.x / R, r = blockIdx.x % R, l = threadIdx.x;
+  const float* S = part + (long long)p.B * p.Hk * splits * R * D;
+  auto row = [&](int s) { return ((long long)inst * splits + s) * R + r; };
+  float M = -INFINITY;
+  for (int s = 0; s < splits; ++s) M = fmaxf(M, S[2 * row(s)]);
+  float L = 0.f, o[D / 64];
+#pragma unroll
+  for (int u = 0; u < D / 64; ++u) o[u] = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const float m = S[2 * row(s)], f = m == -INFINITY ? 0.f : ex2(m - M);
+    L = fmaf(S[2 * row(s) + 1], f, L);
+#pragma unroll
+    for (int u = 0; u < D / 64; ++u) {
+      const float v = part[row(s) * D + u * 64 + l];
+      o[u] = fmaf(v, f, o[u]);
+    }
+  }
+  const int b = inst / p.Hk, head = inst % p.Hk * p.G + r / p.Sq, q = r % p.Sq;
+  const float inv = L != 0.f ? 1.f / L : 0.f;
+  T* O = (T*)p.out + b * p.o_bs + q * p.o_rs + head * D;
+#pragma unroll
+  for (int u = 0; u < D / 64; ++u) O[u * 64 + l] = (T)(o[u] * inv);
+  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + __log2f(L)) * LN2 : INFINITY;
+}
+
 // ------------------------------------------------------------------------------- document runs
 // out[b][i] = [first, end) of the run of equal ids around position i; (0, 0) where the id is negative.
 // One block per row: each thread scans a segment, the block scans the segments' borders.
@@ -827,9 +1064,20 @@ __global__ __launch_bounds__(DT) void doc_spans_kernel(const int* __restrict__ i
   }
 }
 
+// few rows and no dropout: the split form; shares of a cache so that there are about 4 blocks for each of
+// 256 CUs, none below 512 keys
+bool few_rows(int G, int Sq, float p_drop) { return G * (long long)Sq <= 32 && p_drop == 0.f; }
+int few_splits(int inst, int Sk) { return std::max(1, std::min((1024 + inst - 1) / inst, Sk / 512)); }
 template <typename T, int D>
-int launch_fwd(Shaped p, hipStream_t s) {
+int launch_fwd(Shaped p, float* part, hipStream_t s) {
   constexpr int NW = 4;
+  if (few_rows(p.G, p.Sq, p.p_drop)) {
+    const int inst = p.B * p.Hk, splits = few_splits(inst, p.Sk);
+    hipLaunchKernelGGL((shaped_few_kernel<T, D>), dim3((unsigned)(inst * splits)), dim3(FW * 64), 0, s, p, splits, part);
+    if (splits > 1)
+      hipLaunchKernelGGL((shaped_few_join_kernel<T, D>), dim3((unsigned)(inst * p.G * p.Sq)), dim3(64), 0, s, p, splits, part);
+    return hipGetLastError() == hipSuccess ? 0 : -1;
+  }
   p.tiles = (p.G * p.Sqp + NW * 32 - 1) / (NW * 32);
   hipLaunchKernelGGL((shaped_fwd_kernel<T, D, NW>), dim3((unsigned)(p.tiles * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
   return hipGetLastError() == hipSuccess ? 0 : -1;
@@ -863,15 +1111,22 @@ Shaped params(const long long* shape, const long long* st, const int* kv_len, co
 }  // namespace
 
 extern "C" {
+// f32 words of workspace of a forward (0: none)
+long long tfk_shaped_fwd_ws(const long long* shape, float p_drop) {
+  const int B = (int)shape[0], Hk = (int)shape[2], G = (int)(shape[1] / shape[2]), Sq = (int)shape[3];
+  if (!few_rows(G, Sq, p_drop)) return 0;
+  const int splits = few_splits(B * Hk, (int)shape[4]);
+  return splits == 1 ? 0 : (long long)B * Hk * splits * G * Sq * (shape[5] + 2);
+}
 // f16: 0 bf16, 1 f16
 int tfk_shaped_fwd(const void* q, const void* k, const void* v, void* out, float* lse, int f16_, const long long* shape,
                    const long long* strides, const int* kv_len, const int* q_start, const int* prefix_len,
                    const int* docs, const float* slopes, float scale, float cap, int causal, float p_drop,
-                   unsigned long long seed, hipStream_t s) {
+                   unsigned long long seed, float* ws, hipStream_t s) {
   Shaped p = params(shape, strides, kv_len, q_start, prefix_len, docs, slopes, scale, cap, causal, p_drop, seed);
   p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse;
-  if (shape[5] == 64) return f16_ ? launch_fwd<f16, 64>(p, s) : launch_fwd<bf16, 64>(p, s);
-  return f16_ ? launch_fwd<f16, 128>(p, s) : launch_fwd<bf16, 128>(p, s);
+  if (shape[5] == 64) return f16_ ? launch_fwd<f16, 64>(p, ws, s) : launch_fwd<bf16, 64>(p, ws, s);
+  return f16_ ? launch_fwd<f16, 128>(p, ws, s) : launch_fwd<bf16, 128>(p, ws, s);
 }
 // gstrides [dq_bs, dq_rs, dk_bs, dk_rs, dv_bs, dv_rs]; delta: f32 [B, H, Sq] scratch
 int tfk_shaped_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse,

@@ -82,17 +82,26 @@ struct FwdParams {
   u64* pkeys;   // [T][parts][k]
 };
 __device__ __forceinline__ float log_p(float x, float m, float ls) { return m == -INFINITY ? -INFINITY : (x - m) - ls; }
+// the given token's logit (0 where there is none), loaded ahead of the row's reduction
+struct Given {
+  bool use;
+  float x;
+};
 template <typename T>
-__device__ __forceinline__ void write_row(const FwdParams& p, int row, const Stat& st) {
+__device__ __forceinline__ Given given(const FwdParams& p, int row) {
+  const int id = p.ids[row];
+  Given g{id != p.ignore && (unsigned)id < (unsigned)p.V, 0.f};
+  if (g.use) g.x = (float)((const T*)p.x)[(long long)row * p.ld + id];
+  return g;
+}
+__device__ __forceinline__ void write_row(const FwdParams& p, int row, const Stat& st, const Given& g) {
   const bool any = !(st.s == 0.f);  // false: every logit is -inf
   const float ls = any ? logf(st.s) : 0.f, m = any ? st.m : -INFINITY;
   p.norm[2ll * row] = m;
   p.norm[2ll * row + 1] = ls;
   p.lse[row] = m + ls;
   p.ent[row] = any ? ls - st.y / st.s : 0.f;
-  const int id = p.ids[row];
-  const bool use = id != p.ignore && (unsigned)id < (unsigned)p.V;
-  p.logp[row] = use ? log_p((float)((const T*)p.x)[(long long)row * p.ld + id], m, ls) : 0.f;
+  p.logp[row] = g.use ? log_p(g.x, m, ls) : 0.f;
 }
 __device__ __forceinline__ void write_top(const FwdParams& p, int row, int j, u64 key, const Stat& st, float ls) {
   p.top_ids[(long long)row * p.k + j] = key_col(key);
@@ -164,6 +173,7 @@ __device__ __forceinline__ void top_k(const Vec<T> (&v)[NV], const T* x, int V, 
     for (int i = threadIdx.x; i < n; i += NT) {
       const u64 key = sh.key[i];
       int r = 0;
+#pragma unroll 8
       for (int j = 0; j < n; ++j) r += sh.key[j] > key ? 1 : 0;
       if (r < k) put(r, key);
     }
@@ -201,6 +211,8 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(FwdParams p) {
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const T* x = (const T*)p.x + (long long)row * p.ld;
   const int nvec = (p.V + N - 1) / N, v0 = part * p.per, v1 = min(nvec, v0 + p.per);
+  Given gv{false, 0.f};
+  if (p.parts == 1) gv = given<T>(p, row);
   Vec<T> v[NV];
 #pragma unroll
   for (int c = 0; c < NV; ++c) {
@@ -238,7 +250,7 @@ __global__ __launch_bounds__(NT) void logprobs_fwd_kernel(FwdParams p) {
 #pragma unroll
   for (int u = 1; u < NW; ++u) st = join(st, wst[u]);
   if (threadIdx.x == 0) {
-    if (p.parts == 1) write_row<T>(p, row, st);
+    if (p.parts == 1) write_row(p, row, st, gv);
     else p.pstat[(long long)row * p.parts + part] = st;
   }
   if constexpr (TOP) {
@@ -256,10 +268,12 @@ constexpr int JT = 1024;  // candidates staged at a time
 template <typename T, bool TOP>
 __global__ __launch_bounds__(TOP ? NT : 64) void logprobs_join_kernel(FwdParams p) {
   const int row = blockIdx.x;
+  const Given gv = given<T>(p, row);
   const Stat* ps = p.pstat + (long long)row * p.parts;
   Stat st = ps[0];
+#pragma unroll 4
   for (int u = 1; u < p.parts; ++u) st = join(st, ps[u]);
-  if (threadIdx.x == 0) write_row<T>(p, row, st);
+  if (threadIdx.x == 0) write_row(p, row, st, gv);
   if constexpr (TOP) {
     __shared__ u64 keys[JT];
     const float ls = st.s == 0.f ? 0.f : logf(st.s);
@@ -274,6 +288,7 @@ __global__ __launch_bounds__(TOP ? NT : 64) void logprobs_join_kernel(FwdParams 
         __syncthreads();
         for (int j = threadIdx.x; j < m; j += NT) keys[j] = pk[j0 + j];
         __syncthreads();
+#pragma unroll 8
         for (int j = 0; j < m; ++j) r += keys[j] > key ? 1 : 0;
       }
       if (key != 0 && r < p.k) write_top(p, row, r, key, st, ls);

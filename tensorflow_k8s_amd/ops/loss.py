@@ -86,8 +86,6 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, V: int | None = None
     (their entropy and alternatives are computed all the same). -inf logits are classes of probability 0; a
     row of nothing else has logp -inf, entropy 0. NaN or +inf in a row make its results NaN."""
     V, ids = _logprob_args(logits, ids, V, top_k)
-    T = logits.shape[0]
-    dev = logits.device
     if not on_gpu(logits):
         x = logits[:, :V].float()
         m = x.amax(1, keepdim=True)
@@ -103,11 +101,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, V: int | None = None
             ti = torch.sort(x, dim=1, descending=True, stable=True).indices[:, :top_k]
             tl, ti = lp.gather(1, ti), ti.to(torch.int32)
         return TokenLogprobs(logp, ent, (m + ls)[:, 0], tl, ti, torch.cat([m, ls], 1))
-    logp, ent, lse = (torch.empty(T, dtype=torch.float32, device=dev) for _ in range(3))
-    norm = torch.empty(T, 2, dtype=torch.float32, device=dev)
-    tl = torch.empty(T, top_k, dtype=torch.float32, device=dev) if top_k else None
-    ti = torch.empty(T, top_k, dtype=torch.int32, device=dev) if top_k else None
-    lib().logprobs_fwd(logits, ids, V, top_k, ignore_index, logp, ent, lse, norm, tl, ti)
+    logp, ent, lse, norm, tl, ti = lib().logprobs_fwd(logits, ids, V, top_k, ignore_index)
     return TokenLogprobs(logp, ent, lse, tl, ti, norm)
 
 
@@ -144,8 +138,6 @@ def token_logprobs_bwd(logits: torch.Tensor, ids: torch.Tensor, saved: TokenLogp
         out = torch.zeros(T, cols, dtype=logits.dtype)
         out[:, :V] = d.to(logits.dtype)
         return out
-    dx = torch.empty(T, cols, dtype=logits.dtype, device=logits.device)
     c = lambda t: t.contiguous() if t is not None else None  # noqa: E731
-    lib().logprobs_bwd(logits, ids, V, ignore_index, saved.norm, saved.entropy, saved.top_ids if k else None, c(dlogp),
-                       c(dentropy), c(dtop) if k else None, dx)
-    return dx
+    return lib().logprobs_bwd(logits, ids, V, ignore_index, saved.norm, saved.entropy, saved.top_ids if k else None,
+                              c(dlogp), c(dentropy), c(dtop) if k else None)

@@ -188,9 +188,7 @@ def token_order(ids: torch.Tensor, V: int) -> TokenOrder:
         key = torch.where((flat >= 0) & (flat < V), flat, V)
         keys, perm = torch.sort(key, stable=True)
         return TokenOrder(V, perm.to(torch.int32), keys.to(torch.int32))
-    perm, keys = torch.empty_like(flat), torch.empty_like(flat)
-    lib().token_order(flat, V, perm, keys)
-    return TokenOrder(V, perm, keys)
+    return TokenOrder(V, *lib().token_order(flat, V))
 
 
 def embedding_bwd_sorted(order: TokenOrder, dy: torch.Tensor, dword: torch.Tensor, scale: float = 1.0,
@@ -314,9 +312,7 @@ def document_spans(doc_ids: torch.Tensor) -> torch.Tensor:
         raise TypeError(f"document_spans: ids must be int32 [B, S], got {doc_ids.dtype} {tuple(doc_ids.shape)}")
     B, S = doc_ids.shape
     if on_gpu(doc_ids):
-        out = torch.empty(B, S, 2, dtype=torch.int32, device=doc_ids.device)
-        lib().doc_spans(doc_ids.contiguous(), out)
-        return out
+        return lib().doc_spans(doc_ids.contiguous())
     new = torch.ones(B, S, dtype=torch.bool)
     new[:, 1:] = doc_ids[:, 1:] != doc_ids[:, :-1]
     i = torch.arange(S).expand(B, S)
@@ -374,15 +370,17 @@ class AttnSpec:
             raise ValueError(f"attention: scale must be positive, got {self.scale}")
         if self.prefix_len is not None and not self.causal:
             raise ValueError("attention: prefix_len needs causal=True")
-        for n, t, dt, shape in (("kv_len", self.kv_len, torch.int32, (self.B,)), ("q_start", self.q_start, torch.int32, (self.B,)),
-                                ("prefix_len", self.prefix_len, torch.int32, (self.B,)),
+        B = (self.B,)
+        for n, t, dt, shape in (("kv_len", self.kv_len, torch.int32, B), ("q_start", self.q_start, torch.int32, B),
+                                ("prefix_len", self.prefix_len, torch.int32, B),
                                 ("slopes", self.slopes, torch.float32, (self.H,)),
                                 ("docs", self.docs, torch.int32, (self.B, self.Sk, 2))):
-            if t is not None and (t.dtype != dt or tuple(t.shape) != shape or not t.is_contiguous()):
+            if t is not None and (t.dtype is not dt or t.shape != shape or not t.is_contiguous()):
                 raise ValueError(f"attention: {n} must be contiguous {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
-        for n, (buf, col), S, heads in (("q", self.q, self.Sq, self.H), ("k", self.k, self.Sk, self.kv_heads),
-                                        ("v", self.v, self.Sk, self.kv_heads)):
-            _span_check(n, buf, col, self.B, S, heads * self.head_dim)
+        W = self.kv_heads * self.head_dim
+        _span_check("q", *self.q, self.B, self.Sq, self.H * self.head_dim)
+        _span_check("k", *self.k, self.B, self.Sk, W)
+        _span_check("v", *self.v, self.B, self.Sk, W)
 
     def strides(self):
         out = []
@@ -394,16 +392,12 @@ class AttnSpec:
 
 def _span_check(n, buf, col, B, S, W):
     """A (buf, col) operand of shaped attention holds [B, S, W] at column col."""
-    if buf.dtype not in (torch.bfloat16, torch.float16):
+    if buf.dtype is not torch.bfloat16 and buf.dtype is not torch.float16:
         raise TypeError(f"attention: {n} must be bfloat16 or float16, got {buf.dtype}")
-    ok = (buf.dim() == 2 and buf.shape[0] == B * S) or (buf.dim() == 3 and buf.shape[0] == B and buf.shape[1] >= S)
-    if not ok or col < 0 or col + W > buf.shape[-1]:
-        raise ValueError(f"attention: {n} must hold [{B}*{S}, {W}] at column {col}, got {list(buf.shape)}")
-
-
-def _buf_strides(buf, S):
-    """[batch, token] strides of a 2-D [B*S, width] or 3-D [B, S', width] buffer."""
-    return [buf.stride(0), buf.stride(1)] if buf.dim() == 3 else [S * buf.stride(0), buf.stride(0)]
+    sh = buf.shape
+    ok = sh[0] == B * S if len(sh) == 2 else len(sh) == 3 and sh[0] == B and sh[1] >= S
+    if not ok or col < 0 or col + W > sh[-1]:
+        raise ValueError(f"attention: {n} must hold [{B}*{S}, {W}] at column {col}, got {list(sh)}")
 
 
 def _shaped_view(buf, col, B, S, heads, D):
@@ -459,11 +453,7 @@ def _shaped_fwd(sp):
         o, lse = _shaped_ref(sp, *(_shaped_view(b, c, B, S, n, D).float() for (b, c), S, n in
                                    ((sp.q, Sq, H), (sp.k, Sk, Hk), (sp.v, Sk, Hk))))
         return o.reshape(B * Sq, H * D).to(q.dtype), lse
-    out = torch.empty(B * Sq, H * D, dtype=q.dtype, device=q.device)
-    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=q.device)
-    st = _buf_strides(q, Sq) + _buf_strides(sp.k[0], Sk) + _buf_strides(sp.v[0], Sk) + [Sq * H * D, H * D]
-    lib().shaped_fwd(q, sp.q[1], sp.k[0], sp.k[1], sp.v[0], sp.v[1], out, lse, [B, H, Hk, Sq, Sk, D], st, *_shaped_args(sp))
-    return out, lse
+    return lib().shaped_fwd(*sp.q, *sp.k, *sp.v, [B, H, Hk, Sq, Sk, D], *_shaped_args(sp))
 
 
 def _shaped_bwd(sp, out, dout, lse, dq, dk, dv):
@@ -480,11 +470,7 @@ def _shaped_bwd(sp, out, dout, lse, dq, dk, dv):
         for (_, (buf, col), S, n), g in zip(geom, grads):
             _shaped_view(buf, col, B, S, n, D).copy_(g.to(buf.dtype))
         return
-    dout = dout.contiguous()
-    st = _buf_strides(sp.q[0], Sq) + _buf_strides(sp.k[0], Sk) + _buf_strides(sp.v[0], Sk) + [Sq * H * D, H * D]
-    gst = _buf_strides(dq[0], Sq) + _buf_strides(dk[0], Sk) + _buf_strides(dv[0], Sk)
-    lib().shaped_bwd(sp.q[0], sp.q[1], sp.k[0], sp.k[1], sp.v[0], sp.v[1], out, dout, lse, dq[0], dq[1], dk[0], dk[1],
-                     dv[0], dv[1], [B, H, Hk, Sq, Sk, D], st, gst, *_shaped_args(sp))
+    lib().shaped_bwd(*sp.q, *sp.k, *sp.v, out, dout.contiguous(), lse, *dq, *dk, *dv, [B, H, Hk, Sq, Sk, D], *_shaped_args(sp))
 
 
 def attention_fwd(sp: AttnSpec):
