@@ -17,7 +17,8 @@ int tfk_shaped_fwd(const void*, const void*, const void*, void*, float*, int, co
 long long tfk_shaped_fwd_ws(const long long*, float);
 int tfk_shaped_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*,
                    void*, int, const long long*, const long long*, const long long*, const int*, const int*, const int*,
-                   const int*, const float*, float, float, int, float, unsigned long long, hipStream_t);
+                   const int*, const float*, float, float, int, float, unsigned long long, float*, hipStream_t);
+long long tfk_shaped_bwd_ws(const long long*);
 int tfk_doc_spans(const int*, long long, int, int*, hipStream_t);
 int tfk_logprobs_kmax();
 long long tfk_logprobs_ws(long long, int, int, int);
@@ -68,7 +69,7 @@ void check_cols(const torch::Tensor& t, const torch::Tensor& ref, long long off,
   TORCH_CHECK(t.dim() >= 2 && (t.size(-1) == 1 || t.stride(-1) == 1), n, " needs unit stride along its last dim");
   TORCH_CHECK(off >= 0 && off + W <= t.size(-1), n, ": columns ", off, "..", off + W, " outside a width of ", t.size(-1));
   TORCH_CHECK(rs % 8 == 0 && bs % 8 == 0 && off % 8 == 0, n, ": strides/offset must be multiples of 8 elements");
-  TORCH_CHECK(rs >= W || S == 1, n, ": token stride ", rs, " < ", W);
+  TORCH_CHECK((rs >= W || S == 1) && rs < (1 << 23), n, ": token stride ", rs, " not in ", W, "..2^23");
   const long long have = (long long)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
   TORCH_CHECK(bs >= 0 && off + (B - 1) * bs + (S - 1) * rs + W <= have, n, " too small for its shape");
   TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) + 2 * off) % 16 == 0, n, " must be 16-byte aligned");
@@ -170,11 +171,13 @@ void shaped_bwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch:
   check_cols(dv, q, dvo, gs[4], gs[5], B, Sk, Hk * D, true, "dv");
   need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
   const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
-  torch::Tensor delta = at::empty({B * H * Sq}, lse.options());
+  torch::Tensor delta = at::empty({2 * B * H * Sq}, lse.options()), ws;
+  const long long wn = tfk_shaped_bwd_ws(c.sh);
+  if (wn) ws = at::empty({wn}, lse.options());
   check_rc(tfk_shaped_bwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
                           delta.data_ptr<float>(), at(dq, dqo), at(dk, dko), at(dv, dvo), c.f16, c.sh, c.st, gs, m.kv_len,
                           m.q_start, m.prefix, m.docs, m.slopes, (float)scale, (float)cap, causal ? 1 : 0, (float)p_drop,
-                          (unsigned long long)seed, stream_of(q)),
+                          (unsigned long long)seed, wn ? ws.data_ptr<float>() : nullptr, stream_of(q)),
            "shaped_bwd");
 }
 
