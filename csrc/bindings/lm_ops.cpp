@@ -18,7 +18,7 @@ long long tfk_shaped_fwd_ws(const long long*, float);
 int tfk_shaped_bwd(const void*, const void*, const void*, const void*, const void*, const float*, float*, void*, void*,
                    void*, int, const long long*, const long long*, const long long*, const int*, const int*, const int*,
                    const int*, const float*, float, float, int, float, unsigned long long, float*, hipStream_t);
-long long tfk_shaped_bwd_ws(const long long*);
+long long tfk_shaped_bwd_ws(const long long*, float);
 int tfk_doc_spans(const int*, long long, int, int*, hipStream_t);
 int tfk_logprobs_kmax();
 long long tfk_logprobs_ws(long long, int, int, int);
@@ -82,7 +82,7 @@ void check_shape(const std::vector<int64_t>& s, double scale, double cap, double
   TORCH_CHECK(s[1] % s[2] == 0, "heads must be a multiple of key heads");
   TORCH_CHECK(s[5] == 64 || s[5] == 128, "head dim must be 64 or 128, got ", s[5]);
   // query rows padded to whole tiles; block counts and row indices are 32-bit
-  TORCH_CHECK((s[3] + 128) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x3fffffff, "sequence too long");
+  TORCH_CHECK((s[3] + 128) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x7ffffff, "sequence too long");
   TORCH_CHECK(((s[3] + 128) / 32 * (s[1] / s[2]) + s[4] / 64 + 2) * s[0] * s[2] <= 0x7fffffff, "attention grid too large");
   TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "scale must be positive, got ", scale);
   TORCH_CHECK(cap >= 0.0 && std::isfinite(cap), "softcap must be >= 0, got ", cap);
@@ -172,7 +172,7 @@ void shaped_bwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch:
   need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
   const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
   torch::Tensor delta = at::empty({2 * B * H * Sq}, lse.options()), ws;
-  const long long wn = tfk_shaped_bwd_ws(c.sh);
+  const long long wn = tfk_shaped_bwd_ws(c.sh, (float)p_drop);
   if (wn) ws = at::empty({wn}, lse.options());
   check_rc(tfk_shaped_bwd(at(q, qo), at(k, ko), at(v, vo), out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
                           delta.data_ptr<float>(), at(dq, dqo), at(dk, dko), at(dv, dvo), c.f16, c.sh, c.st, gs, m.kv_len,

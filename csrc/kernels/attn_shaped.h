@@ -1,0 +1,380 @@
+// Attention with shaped scores for gfx950: forward, dQ pass, dK/dV pass (flash style, no float atomics).
+//
+//   s(i, j) = cap tanh(scale q_i.k_j / cap) - slope_h |p_i - j|          (cap, slopes: optional)
+//   key j is seen by query i iff lo_i <= j < hi_i;  P = softmax over the seen keys, O = P V
+//
+// p_i = i + q_start[b] is the query's position among the keys. Every mask here is one interval of keys
+// per query: hi = min(kv_len, Sk), causal: hi <= p + 1 or, with a prefix, hi <= max(p + 1, prefix_len);
+// documents: [lo, hi) also within the run of the query's document. So a block walks exactly the key
+// tiles between its rows' smallest lo and largest hi, a tile that all rows of a wave see needs no mask
+// arithmetic, and no [Sq, Sk] mask is read. A query that sees no key gets O = 0 and lse = +inf (its P
+// and gradients vanish); rows that no query sees are zeroed on their way into the LDS, so what padding
+// holds never meets a product.
+//
+// Heads: H query heads in Hk groups of G = H / Hk. The forward and dQ passes lay the G heads of a group
+// out as G * Sqp rows (queries fastest; Sqp: Sq, padded), so few queries of many heads share one tile;
+// the dK/dV pass sums a group's heads in its registers.
+//
+// Types bf16 / f16, head dim D = 64 / 128, any token and batch strides (multiples of 8 elements).
+//
+// MFMA mapping (32x32x16, wave64): mfma(X, Y) gives lane l, slot r: sum_k X[(r & 3) + 8 (r >> 2) + 4 (l >> 5)][k]
+// * Y[l & 31][k], operand fragments put row (l & 31), k-slots 8 (l >> 5) .. + 7 in lane l. The streamed
+// tile is X (rows of K and V, or of Q and dO in the dK/dV pass), the lane's own row is Y: a lane owns one
+// query (key), row statistics are lane scalars plus one exchange with lane ^ 32. The slots of two 4-row
+// groups are, packed, the k-slots of the next product's Y operand when its X operand (V^T, K^T, dO^T, Q^T)
+// is read with the same row order: two ds_read_b64_tr_b16 of rows 4h.. and 8 + 4h.. of each 16.
+// LDS rows are D elements, their 16-byte chunks XOR-swizzled (swz): conflict-free for both reads.
+#pragma once
+#include "common.h"
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+typedef _Float16 f16;
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+template <bool B>
+using bconst = std::integral_constant<bool, B>;
+template <int I>
+using iconst = std::integral_constant<int, I>;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// streamed rows of a tile
+constexpr int key_tile(int D) { return 64; }    // forward, dQ
+constexpr int query_tile(int D) { return 64; }  // dK/dV
+constexpr float RAISE = 8.f;  // log2 units by which a row may outgrow its running maximum
+
+template <typename T>
+struct Ty;
+template <>
+struct Ty<bf16> {
+  typedef bf16x8 x8;
+  typedef bf16x4 x4;
+  static __device__ __forceinline__ f32x16 mfma(x8 x, x8 y, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ x4 tr(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS x4*)p); }
+};
+template <>
+struct Ty<f16> {
+  typedef f16x8 x8;
+  typedef f16x4 x4;
+  static __device__ __forceinline__ f32x16 mfma(x8 x, x8 y, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ x4 tr(const char* p) {  // 16-bit elements move as they are
+    return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p));
+  }
+};
+
+struct Shaped {
+  const void *q, *k, *v, *o, *dout;
+  void *out, *dq, *dk, *dv;
+  float *lse, *delta;  // delta [2][B][H][Sq]: lse in log2 units, -rowsum(dO * O)
+  long long q_bs, k_bs, v_bs, o_bs, dq_bs, dk_bs, dv_bs;  // batch strides (elements)
+  long long q_rs, k_rs, v_rs, o_rs, dq_rs, dk_rs, dv_rs;  // token strides
+  int B, H, Hk, G, Sq, Sk, Sqp, tiles;                    // tiles: row tiles of one (batch, key head)
+  const int *kv_len, *q_start, *prefix_len;               // [B] or null
+  const int2* docs;                                       // [B][Sk] document run of each position, or null
+  const float* slopes;                                    // [H] or null
+  float scale, cap;
+  int causal, remap;
+  float p_drop;
+  unsigned long long seed;
+  const unsigned long long* seed_key;
+};
+
+// the score rules of a call, compiled in: as runtime branches their joins cost the dK/dV pass 40 registers
+template <bool DOCS, bool CAP, bool BIAS, bool DROP>
+struct Rules {
+  static constexpr bool docs = DOCS, cap = CAP, bias = BIAS, drop = DROP;
+};
+template <typename F>
+void with_rules(const Shaped& p, F f) {
+  auto dr = [&](auto docs, auto cap, auto bias) {
+    if (p.p_drop > 0.f) f(Rules<docs.value, cap.value, bias.value, true>{});
+    else f(Rules<docs.value, cap.value, bias.value, false>{});
+  };
+  auto bi = [&](auto docs, auto cap) {
+    if (p.slopes) dr(docs, cap, bconst<true>{});
+    else dr(docs, cap, bconst<false>{});
+  };
+  auto ca = [&](auto docs) {
+    if (p.cap > 0.f) bi(docs, bconst<true>{});
+    else bi(docs, bconst<false>{});
+  };
+  if (p.docs) ca(bconst<true>{});
+  else ca(bconst<false>{});
+}
+
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float pair_max(float v) {  // over lanes l, l ^ 32
+  float o;
+  const float a = lane_swap32(v, o);
+  return fmaxf(a, o);
+}
+// wave-wide integer extremes by DPP and permlane swaps (common.h wave_sum's butterfly)
+template <int CTRL>
+__device__ __forceinline__ int dpp_i(int v) {
+  return __builtin_amdgcn_mov_dpp(v, CTRL, 0xf, 0xf, false);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+  v = max(v, dpp_i<0xB1>(v));
+  v = max(v, dpp_i<0x4E>(v));
+  v = max(v, dpp_i<0x141>(v));
+  v = max(v, dpp_i<0x140>(v));
+  auto a = __builtin_amdgcn_permlane16_swap((unsigned)v, (unsigned)v, false, false);
+  v = max((int)a[0], (int)a[1]);
+  auto b = __builtin_amdgcn_permlane32_swap((unsigned)v, (unsigned)v, false, false);
+  return __builtin_amdgcn_readfirstlane(max((int)b[0], (int)b[1]));
+}
+__device__ __forceinline__ int wave_min_i(int v) { return ~wave_max_i(~v); }
+// LDS-only block barrier: the next tile's global loads stay in flight across it
+__device__ __forceinline__ void lds_bar() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// ---- masks
+struct Span {
+  int lo, hi;  // lo >= hi: sees nothing
+};
+// one batch's mask: query i at position i + shift sees keys below min(kvl, causal: max(position + 1, prefix))
+struct Mask {
+  int shift, kvl, prefix;
+  bool causal;
+  const int2* docs;
+  int Sk;
+  __device__ __forceinline__ Mask(const Shaped& p, int b) {
+    shift = p.q_start ? min(max(p.q_start[b], -(1 << 30)), 1 << 30) : 0;
+    kvl = min(p.kv_len ? p.kv_len[b] : p.Sk, p.Sk);
+    prefix = p.prefix_len ? p.prefix_len[b] : 0;
+    causal = p.causal != 0;
+    docs = p.docs ? p.docs + (long long)b * p.Sk : nullptr;
+    Sk = p.Sk;
+  }
+  // d: the document run at the query's position (DOCS)
+  template <bool DOCS>
+  __device__ __forceinline__ Span of(int q, int2 d) const {
+    const int pos = q + shift;
+    Span s{0, causal ? min(kvl, max(pos + 1, prefix)) : kvl};
+    if (DOCS) {
+      s.lo = max(0, d.x);
+      s.hi = pos >= 0 && pos < Sk ? min(s.hi, d.y) : 0;
+    }
+    if (s.hi <= s.lo) s.lo = s.hi = 0;
+    return s;
+  }
+  __device__ __forceinline__ int2 doc_at(int pos) const { return docs[min(max(pos, 0), Sk - 1)]; }
+  template <bool DOCS>
+  __device__ __forceinline__ Span of(int q) const {
+    return of<DOCS>(q, DOCS ? doc_at(q + shift) : int2{0, 0});
+  }
+  // positions that see key j < Sk: [lo, hi) (superset; the pair test decides)
+  template <bool DOCS>
+  __device__ __forceinline__ Span seen_by(int j) const {
+    Span s{-(1 << 30), 0x7fffffff};
+    if (j >= kvl) return Span{0, 0};
+    if (DOCS) {
+      const int2 d = docs[j];
+      if (d.y <= d.x) return Span{0, 0};
+      s.lo = d.x;
+      s.hi = d.y;
+    }
+    if (causal && j >= prefix) s.lo = max(s.lo, j);
+    return s;
+  }
+};
+
+// ---- dropout: the mask bytes of attention.hip (one hash per 4 queries and key), see dropout_keep_mask
+__device__ __forceinline__ uint32_t head_seed(const Shaped& p, int bh) {
+  const unsigned long long s = eff_seed(p.seed, p.seed_key);
+  return hash32((uint32_t)s ^ (uint32_t)(s >> 32) ^ ((uint32_t)bh * 0x9E3779B9u));
+}
+__device__ __forceinline__ int drop_thr(float p) {
+  const int t = (int)(p * 256.f + 0.5f);
+  return t > 255 ? 255 : t;
+}
+template <int R>
+__device__ __forceinline__ uint32_t qb(uint32_t h) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)h, R * 0x55, 0xf, 0xf, false);
+}
+// keep bits of this lane's query with keys kb .. kb + 3; a lane quad holds the 4 queries of a group
+__device__ __forceinline__ unsigned keep4_rows(uint32_t hs, int qg, int kb, int j, int thr) {
+  const uint32_t h = hash32(hs ^ (uint32_t)(qg + kb + j));
+  const uint32_t h0 = qb<0>(h), h1 = qb<1>(h), h2 = qb<2>(h), h3 = qb<3>(h);
+  const int sh = 8 * j;
+  return (((h0 >> sh) & 0xffu) >= (uint32_t)thr ? 1u : 0u) | (((h1 >> sh) & 0xffu) >= (uint32_t)thr ? 2u : 0u) |
+         (((h2 >> sh) & 0xffu) >= (uint32_t)thr ? 4u : 0u) | (((h3 >> sh) & 0xffu) >= (uint32_t)thr ? 8u : 0u);
+}
+// keep bits of this lane's key with queries 4 qg .. + 3
+__device__ __forceinline__ unsigned keep4_cols(uint32_t hs, int qg, int Sk, int key, int thr) {
+  const uint32_t h = hash32(hs ^ (uint32_t)(qg * Sk + key));
+  return ((h & 0xffu) >= (uint32_t)thr ? 1u : 0u) | (((h >> 8) & 0xffu) >= (uint32_t)thr ? 2u : 0u) |
+         (((h >> 16) & 0xffu) >= (uint32_t)thr ? 4u : 0u) | ((h >> 24) >= (uint32_t)thr ? 8u : 0u);
+}
+
+// ---- LDS tiles: [rows][D], 16-byte chunk c of row r at chunk c ^ swz(r)
+template <int D>
+__device__ __forceinline__ int swz(int r) {
+  return D == 64 ? (((r >> 1) & 1) << 2) | ((r >> 2) & 3) : ((r & 3) << 2) | ((r >> 2) & 3);
+}
+// Per-lane LDS byte addresses of the fragment reads. Row blocks and the slot of a double-buffered tile are
+// immediate offsets on top (the tile loops are unrolled by the slot): no address arithmetic in the loops,
+// which are bound by vector instructions.
+template <int D>
+struct Offs {
+  int row[D / 16];    // row (l & 31), k-slots 16 kk + 8 h ..
+  int tr[D / 32][2];  // column 32 db + (l & 31), rows 4 h .. and 8 + 4 h .. of a 16-row group
+  __device__ __forceinline__ void init() {
+    const int l = threadIdx.x & 63, h = l >> 5, r = l & 31;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) row[kk] = r * (2 * D) + (((2 * kk + h) ^ swz<D>(r)) << 4);
+    const int li = l & 15, t = 4 * h + (li >> 2), c = 2 * ((l >> 4) & 1) + ((li & 3) >> 1);
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        tr[db][u] = (t + 8 * u) * (2 * D) + (((4 * db + c) ^ swz<D>(t + 8 * u)) << 4) + (li & 1) * 8;
+  }
+};
+// rows 32 rb + (l & 31), k-slots 16 kk + 8 h .. of the tile at byte `at` of `lds`
+template <typename T, int D>
+__device__ __forceinline__ typename Ty<T>::x8 frag_row(const char* lds, int at, const Offs<D>& o, int rb, int kk) {
+  return *(const typename Ty<T>::x8*)(lds + o.row[kk] + (at + rb * 32 * 2 * D));
+}
+// X operand of a product over 16 tile rows (16 kc ..): column 32 db + (l & 31)
+template <typename T, int D>
+__device__ __forceinline__ typename Ty<T>::x8 frag_tr(const char* lds, int at, const Offs<D>& o, int kc, int db) {
+  typename Ty<T>::x8 r;
+  r.lo = Ty<T>::tr(lds + o.tr[db][0] + (at + kc * 16 * 2 * D));
+  r.hi = Ty<T>::tr(lds + o.tr[db][1] + (at + kc * 16 * 2 * D));
+  return r;
+}
+// k-slots 16 kk + 8 h .. of a row in memory, zeros unless ok
+template <typename T>
+__device__ __forceinline__ typename Ty<T>::x8 frag_mem(const T* row, int kk, bool ok) {
+  const int h = (threadIdx.x & 63) >> 5;
+  const u32x4 v = *(const u32x4*)(row + kk * 16 + 8 * h);
+  const u32x4 z = u32x4{0u, 0u, 0u, 0u};
+  return __builtin_bit_cast(typename Ty<T>::x8, ok ? v : z);
+}
+template <typename T>
+__device__ __forceinline__ typename Ty<T>::x8 pack8(const f32x16& a, int half) {
+  typename Ty<T>::x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)a[8 * half + e];
+  return r;
+}
+
+// A tile of KT rows of D elements from memory straight into the LDS (buffer loads with LDS destination, 16
+// bytes a lane): instruction i of wave w fills rows (i NW + w) RPI .. + RPI - 1, the swizzle is in the
+// lanes' source addresses. Rows from `rows` on lie past the descriptor's end and arrive as zeros.
+//
+// Tiles are double-buffered: tile t + 1 is issued before tile t's products, each wave waits for its own loads
+// behind them (dma_wait), clears rows of its own that nothing sees (DeadRows), and a barrier hands the tile
+// over. (Rings of 3 and 4 smaller tiles measured slower: B1 H16/4 S8192 D128 capped 1956 us against 1755.)
+// descriptor of `rows` rows, rb bytes apart, from a block-uniform address
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const void* base, int rb, int rows) {
+  const unsigned long long a = (unsigned long long)base;
+  const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)a), hi = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(((unsigned long long)hi << 32) | lo), (short)0,
+                                           __builtin_amdgcn_readfirstlane(rows * rb), 0x00020000);
+}
+__device__ __forceinline__ void dma_b128(__amdgpu_buffer_rsrc_t r, unsigned lds, unsigned voff, unsigned soff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff),
+               "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff)) : "memory");
+}
+__device__ __forceinline__ void dma_b32(__amdgpu_buffer_rsrc_t r, unsigned lds, unsigned voff) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r) : "memory");
+}
+__device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+template <int D, int NW, int KT>
+struct Dma {
+  static constexpr int N = KT * D * 2 / (NW * 1024), RPI = 512 / D, STEP = NW * RPI;
+  static_assert(N >= 1 && (N == 1 || STEP % 16 == 0), "one swizzle for all instructions of a lane");
+  unsigned voff, step;  // lane's byte offset of instruction 0, bytes between instructions
+  int row0;
+  __device__ __forceinline__ void init(long long rs) {
+    const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+    row0 = w * RPI + l / (D / 8);
+    voff = (unsigned)(row0 * (int)rs * 2 + (((l % (D / 8)) ^ swz<D>(row0)) << 4));
+    step = (unsigned)(STEP * (int)rs * 2);
+  }
+  __device__ __forceinline__ int row(int i) const { return row0 + i * STEP; }
+  template <typename T>
+  __device__ __forceinline__ void issue(const T* base, long long rs, int rows, unsigned lds) const {
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const __amdgpu_buffer_rsrc_t rsrc = rows_rsrc(base, (int)rs * 2, max(min(rows, KT), 0));
+#pragma unroll
+    for (int i = 0; i < N; ++i) dma_b128(rsrc, lds + (i * NW + w) * 1024, voff, i * step);
+  }
+  // zeros over this lane's piece of instruction i
+  __device__ __forceinline__ void clear(char* tile, int i) const {
+    *(u32x4*)(tile + (i * NW + (int)(threadIdx.x >> 6)) * 1024 + (threadIdx.x & 63) * 16) = u32x4{0u, 0u, 0u, 0u};
+  }
+};
+
+// ---- scores: raw products s -> exponents of 2
+// plain: x = s scale log2e. Capped: cap tanh(u) = cap - 2 cap r with r = 1 / (1 + e^2u), u = s scale / cap; the
+// constant cap shifts a whole row, so x = -2 cap log2e r, and d tanh = 1 - tanh^2 = 4 (r - r^2). Distances add
+// -slope log2e |p - j|. (Row statistics between the passes are in these shifted units.)
+template <typename O>
+struct Score {
+  float c2, c2l, mult, base;  // 2 log2e scale / cap, -2 cap log2e, scale log2e, the shift
+  __device__ __forceinline__ Score(const Shaped& p) {
+    mult = p.scale * LOG2E;
+    c2 = O::cap ? 2.f * mult / p.cap : 0.f;
+    base = O::cap ? p.cap * LOG2E : 0.f;
+    c2l = -2.f * base;
+  }
+  // native exp2 and reciprocal: saturates through e = inf (r = 0) and e = 0 (r = 1)
+  __device__ __forceinline__ float r(float s) const { return __builtin_amdgcn_rcpf(1.f + ex2(s * c2)); }
+};
+// slot r of a 32-row block: row (r & 3) + 8 (r >> 2) (+ 4 h)
+__device__ __forceinline__ constexpr int srow(int r) { return (r & 3) + 8 * (r >> 2); }
+
+// slots whose row is not in [0, len) from `base` take v. `base` is made opaque so that the compares stay inside the
+// branch of the partly visible tiles (hoisted, they cost every tile 32 instructions).
+__device__ __forceinline__ void mask_slots(f32x16& s, unsigned base, unsigned len, float v) {
+  asm volatile("" : "+v"(base));
+#pragma unroll
+  for (int e = 0; e < 16; ++e) s[e] = base + (unsigned)srow(e) < len ? s[e] : v;
+}
+
+// block -> (key-head instance, row tile); blocks of one instance share an XCD's L2 where there are
+// enough instances, later (causal: longer) tiles first
+__device__ __forceinline__ void locate(const Shaped& p, int n, bool rev, int& inst, int& tile) {
+  const int id = p.remap ? xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
+  inst = id / n;
+  tile = id % n;
+  if (rev) tile = n - 1 - tile;
+}
+
+// what a wave's rows see: union [ulo, uhi) and intersection [ilo, ihi)
+struct Reach {
+  int ulo, uhi, ilo, ihi;
+  __device__ __forceinline__ Reach(const Span& s, bool sees) {
+    ulo = wave_min_i(sees ? s.lo : 0x7fffffff);
+    uhi = wave_max_i(sees ? s.hi : 0);
+    ilo = wave_max_i(sees ? s.lo : 0);
+    ihi = wave_min_i(sees ? s.hi : 0x7fffffff);
+  }
+};
+// With documents: one 4-byte mark for each staged row of the lane, loaded into the wave's own LDS words
+// beside the tile; rows whose mark says that nothing sees them are cleared.
+template <int D, int NW, int KT>
+struct DeadRows {
+  static constexpr int N = Dma<D, NW, KT>::N, WORDS = N * NW * 64;  // of one slot
+  // marks at base[row * stride_b bytes + at], rows outside [0, rows) read 0
+  static __device__ __forceinline__ void issue(const void* base, int stride, int at, int rows, int row0, const Dma<D, NW, KT>& m, unsigned lds) {
+    const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, stride, rows);
+    const int w = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < N; ++i) dma_b32(r, lds + (i * NW + w) * 256, (unsigned)((row0 + m.row(i)) * stride + at));
+  }
+  static __device__ __forceinline__ unsigned mark(const unsigned* slot, int i) { return slot[(i * NW) * 64 + threadIdx.x]; }
+};
+}  // namespace
