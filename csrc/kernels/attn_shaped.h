@@ -74,12 +74,13 @@ struct Shaped {
   float *lse, *delta;  // delta [2][B][H][Sq]: lse in log2 units, -rowsum(dO * O)
   long long q_bs, k_bs, v_bs, o_bs, dq_bs, dk_bs, dv_bs;  // batch strides (elements)
   long long q_rs, k_rs, v_rs, o_rs, dq_rs, dk_rs, dv_rs;  // token strides
-  int B, H, Hk, G, Sq, Sk, Sqp, tiles;                    // tiles: row tiles of one (batch, key head)
+  int B, H, Hk, G, Sq, Sk, Sqp;
+  int tiles, heads;  // row tiles of a column, columns of one (batch, key head): G where a head fills whole tiles, else 1
   const int *kv_len, *q_start, *prefix_len;               // [B] or null
   const int2* docs;                                       // [B][Sk] document run of each position, or null
   const float* slopes;                                    // [H] or null
   float scale, cap;
-  int causal, remap;
+  int causal;
   float p_drop;
   unsigned long long seed;
   const unsigned long long* seed_key;
@@ -344,13 +345,19 @@ __device__ __forceinline__ void mask_slots(f32x16& s, unsigned base, unsigned le
   for (int e = 0; e < 16; ++e) s[e] = base + (unsigned)srow(e) < len ? s[e] : v;
 }
 
-// block -> (key-head instance, row tile); blocks of one instance share an XCD's L2 where there are
-// enough instances, later (causal: longer) tiles first
-__device__ __forceinline__ void locate(const Shaped& p, int n, bool rev, int& inst, int& tile) {
-  const int id = p.remap ? xcd_remap(blockIdx.x, gridDim.x) : (int)blockIdx.x;
-  inst = id / n;
-  tile = id % n;
-  if (rev) tile = n - 1 - tile;
+// Blocks of one launch: the tile's rank is the slow index, the columns (head instances) the fast one. Consecutive
+// blocks go round the 8 XCDs, so a column stays on one XCD (8 divides their number, usually) and its K / V in
+// that XCD's L2, every XCD and CU gets tiles of all ranks, and the long ones (causal: the last rows, the
+// first keys) start first. (A column's tiles side by side instead: CUs were idle 57% of a packed-document
+// forward, the tiles of one CU being all long or all short.)
+__device__ __forceinline__ void locate(int columns, int& column, int& rank) {
+  rank = (int)blockIdx.x / columns;
+  column = (int)blockIdx.x % columns;
+}
+
+inline void row_tiles(Shaped& p, int rows) {
+  p.heads = p.Sqp % rows == 0 ? p.G : 1;
+  p.tiles = (p.G / p.heads * p.Sqp + rows - 1) / rows;
 }
 
 // what a wave's rows see: union [ulo, uhi) and intersection [ilo, ihi)

@@ -64,7 +64,6 @@ Shaped params(const long long* shape, const long long* st, const int* kv_len, co
   // rows of a head: whole tiles where a head has many queries (a tile then walks one head's keys),
   // packed where it has few; dropout hashes quads of queries, so quads stay whole
   p.Sqp = p.Sq >= 64 ? (p.Sq + 127) / 128 * 128 : (p_drop > 0.f ? (p.Sq + 3) / 4 * 4 : p.Sq);
-  p.remap = p.B * p.H >= 8;
   return p;
 }
 }  // namespace

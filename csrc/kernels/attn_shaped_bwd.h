@@ -18,9 +18,10 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
   Offs<D> fo;
   fo.init();
-  int inst, tile;
-  locate(p, p.tiles, p.causal, inst, tile);
-  const int b = inst / p.Hk, hk = inst % p.Hk;
+  int col, rank;
+  locate(p.B * p.Hk * p.heads, col, rank);
+  const int inst = col / p.heads, b = inst / p.Hk, hk = inst % p.Hk;
+  const int tile = col % p.heads * p.tiles + (p.causal ? p.tiles - 1 - rank : rank);
   const int r = tile * NW * 32 + w * 32 + (l & 31), g = r / p.Sqp, q = r % p.Sqp;
   const bool valid = g < p.G && q < p.Sq;
   const int head = hk * p.G + min(g, p.G - 1), qc = min(q, p.Sq - 1);
@@ -193,12 +194,9 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
   Offs<D> fo;
   fo.init();
-  const int nkt = (p.Sk + NW * 32 - 1) / (NW * 32);
-  int inst, tile;
-  locate(p, nkt * splits, false, inst, tile);
-  const int split = tile % splits;
-  tile /= splits;
-  const int b = inst / p.Hk, hk = inst % p.Hk;
+  int col, tile;
+  locate(p.B * p.Hk * splits, col, tile);
+  const int split = col % splits, inst = col / splits, b = inst / p.Hk, hk = inst % p.Hk;
   const int key = tile * NW * 32 + w * 32 + (l & 31);
   const Mask mk(p, b);
   // the queries that see this lane's key: [qlo, qhi)
@@ -445,9 +443,9 @@ int dkv_splits(long long blocks, int G, int Sq) {
 template <typename T, int D>
 int launch_dq(Shaped p, hipStream_t s) {
   constexpr int NW = 4;
-  p.tiles = (p.G * p.Sqp + NW * 32 - 1) / (NW * 32);
+  row_tiles(p, NW * 32);
   with_rules(p, [&](auto o) {
-    hipLaunchKernelGGL((shaped_dq_kernel<T, D, NW, decltype(o)>), dim3((unsigned)(p.tiles * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
+    hipLaunchKernelGGL((shaped_dq_kernel<T, D, NW, decltype(o)>), dim3((unsigned)(p.tiles * p.heads * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
   });
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }

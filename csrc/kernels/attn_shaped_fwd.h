@@ -18,9 +18,10 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
   const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), h = l >> 5;
   Offs<D> fo;
   fo.init();
-  int inst, tile;
-  locate(p, p.tiles, p.causal, inst, tile);
-  const int b = inst / p.Hk, hk = inst % p.Hk;
+  int col, rank;
+  locate(p.B * p.Hk * p.heads, col, rank);
+  const int inst = col / p.heads, b = inst / p.Hk, hk = inst % p.Hk;
+  const int tile = col % p.heads * p.tiles + (p.causal ? p.tiles - 1 - rank : rank);
   const int r = tile * NW * 32 + w * 32 + (l & 31), g = r / p.Sqp, q = r % p.Sqp;
   const bool valid = g < p.G && q < p.Sq;
   const int head = hk * p.G + min(g, p.G - 1), qc = min(q, p.Sq - 1);
@@ -426,9 +427,9 @@ int launch_fwd(Shaped p, float* part, hipStream_t s) {
       hipLaunchKernelGGL((shaped_few_join_kernel<T, D>), dim3((unsigned)(inst * p.G * p.Sq)), dim3(64), 0, s, p, splits, part);
     return hipGetLastError() == hipSuccess ? 0 : -1;
   }
-  p.tiles = (p.G * p.Sqp + NW * 32 - 1) / (NW * 32);
+  row_tiles(p, NW * 32);
   with_rules(p, [&](auto o) {
-    hipLaunchKernelGGL((shaped_fwd_kernel<T, D, NW, decltype(o)>), dim3((unsigned)(p.tiles * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
+    hipLaunchKernelGGL((shaped_fwd_kernel<T, D, NW, decltype(o)>), dim3((unsigned)(p.tiles * p.heads * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
   });
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }
