@@ -355,6 +355,16 @@ __device__ __forceinline__ void locate(int columns, int& column, int& rank) {
   column = (int)blockIdx.x % columns;
 }
 
+// waves of 32 rows in a block of the forward and of the dQ pass. 4; at D = 128, where a CU holds 8 waves, all 8
+// in one block that reads each key tile once instead of twice, if there are 512 such blocks (B1 H16/4 S8192:
+// forward 358 -> 346 us, dQ 459 -> 417 us; with fewer blocks the longest tiles end late, and at D = 64, with 12
+// to 16 waves a CU, 8 were slower: forward 27.8 -> 30.1, dQ 35.4 -> 44.5 us for B4 H16 S2048 in documents of
+// about 512). Dropout's instances keep 4.
+__host__ __device__ constexpr int max_row_waves(int D, bool drop) { return D == 128 && !drop ? 8 : 4; }
+inline int row_waves(const Shaped& p, int D) {
+  return max_row_waves(D, p.p_drop > 0.f) == 8 && p.B * (long long)p.H * (p.Sq / 256) >= 512 ? 8 : 4;
+}
+
 inline void row_tiles(Shaped& p, int rows) {
   p.heads = p.Sqp % rows == 0 ? p.G : 1;
   p.tiles = (p.G / p.heads * p.Sqp + rows - 1) / rows;

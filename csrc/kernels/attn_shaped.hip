@@ -60,10 +60,11 @@ Shaped params(const long long* shape, const long long* st, const int* kv_len, co
   p.q_bs = st[0]; p.q_rs = st[1]; p.k_bs = st[2]; p.k_rs = st[3];
   p.v_bs = st[4]; p.v_rs = st[5]; p.o_bs = st[6]; p.o_rs = st[7];
   p.kv_len = kv_len; p.q_start = q_start; p.prefix_len = prefix_len; p.docs = (const int2*)docs; p.slopes = slopes;
-  p.scale = scale; p.cap = cap; p.causal = causal; p.p_drop = p_drop; p.seed = seed; p.seed_key = tfk_seed_key();
+  p.p_drop = p_drop; p.scale = scale; p.cap = cap; p.causal = causal; p.seed = seed; p.seed_key = tfk_seed_key();
   // rows of a head: whole tiles where a head has many queries (a tile then walks one head's keys),
   // packed where it has few; dropout hashes quads of queries, so quads stay whole
-  p.Sqp = p.Sq >= 64 ? (p.Sq + 127) / 128 * 128 : (p_drop > 0.f ? (p.Sq + 3) / 4 * 4 : p.Sq);
+  const int tile = row_waves(p, (int)shape[5]) * 32;
+  p.Sqp = p.Sq >= 64 ? (p.Sq + tile - 1) / tile * tile : (p_drop > 0.f ? (p.Sq + 3) / 4 * 4 : p.Sq);
   return p;
 }
 }  // namespace

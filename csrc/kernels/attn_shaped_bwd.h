@@ -436,16 +436,20 @@ __global__ __launch_bounds__(256) void shaped_dkv_join_kernel(Shaped p, int spli
   *(typename Ty<T>::x4*)d = v;
 }
 
-// shares of a key tile's queries: about 4 blocks for each of 256 CUs, none below 1024 queries
+// shares of a key tile's queries: about 2 blocks for each of 256 CUs (4 cost
+// B1 H16/4 S8192 D128 50 us more, the join's f32 parts), none below 1024 queries
 int dkv_splits(long long blocks, int G, int Sq) {
-  return (int)std::max(1ll, std::min((1024 + blocks - 1) / blocks, (long long)G * ((Sq + 63) / 64) / 16));
+  return (int)std::max(1ll, std::min((512 + blocks - 1) / blocks, (long long)G * ((Sq + 63) / 64) / 16));
 }
 template <typename T, int D>
 int launch_dq(Shaped p, hipStream_t s) {
-  constexpr int NW = 4;
-  row_tiles(p, NW * 32);
+  const int waves = row_waves(p, D);
+  row_tiles(p, waves * 32);
+  const dim3 grid((unsigned)(p.tiles * p.heads * p.B * p.Hk)), block(waves * 64);
   with_rules(p, [&](auto o) {
-    hipLaunchKernelGGL((shaped_dq_kernel<T, D, NW, decltype(o)>), dim3((unsigned)(p.tiles * p.heads * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
+    constexpr int MAX = max_row_waves(D, decltype(o)::drop);
+    if (waves == MAX) hipLaunchKernelGGL((shaped_dq_kernel<T, D, MAX, decltype(o)>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((shaped_dq_kernel<T, D, 4, decltype(o)>), grid, block, 0, s, p);
   });
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }

@@ -415,7 +415,6 @@ bool few_rows(int G, int Sq, float p_drop) { return G * (long long)Sq <= 32 && p
 int few_splits(int inst, int Sk) { return std::max(1, std::min((1024 + inst - 1) / inst, Sk / 512)); }
 template <typename T, int D>
 int launch_fwd(Shaped p, float* part, hipStream_t s) {
-  constexpr int NW = 4;
   if (few_rows(p.G, p.Sq, p.p_drop)) {
     const int inst = p.B * p.Hk, splits = few_splits(inst, p.Sk);
     with_rules(p, [&](auto o) {
@@ -427,9 +426,13 @@ int launch_fwd(Shaped p, float* part, hipStream_t s) {
       hipLaunchKernelGGL((shaped_few_join_kernel<T, D>), dim3((unsigned)(inst * p.G * p.Sq)), dim3(64), 0, s, p, splits, part);
     return hipGetLastError() == hipSuccess ? 0 : -1;
   }
-  row_tiles(p, NW * 32);
+  const int waves = row_waves(p, D);
+  row_tiles(p, waves * 32);
+  const dim3 grid((unsigned)(p.tiles * p.heads * p.B * p.Hk)), block(waves * 64);
   with_rules(p, [&](auto o) {
-    hipLaunchKernelGGL((shaped_fwd_kernel<T, D, NW, decltype(o)>), dim3((unsigned)(p.tiles * p.heads * p.B * p.Hk)), dim3(NW * 64), 0, s, p);
+    constexpr int MAX = max_row_waves(D, decltype(o)::drop);
+    if (waves == MAX) hipLaunchKernelGGL((shaped_fwd_kernel<T, D, MAX, decltype(o)>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((shaped_fwd_kernel<T, D, 4, decltype(o)>), grid, block, 0, s, p);
   });
   return hipGetLastError() == hipSuccess ? 0 : -1;
 }

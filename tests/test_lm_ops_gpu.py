@@ -137,6 +137,11 @@ ATTN = {
     "dropout_shared": lambda: Case(B=1, H=4, Hk=2, D=128, Sq=35, Sk=70, p_drop=0.5, fused=False),
     "large_scores": lambda: Case(B=1, H=2, Hk=1, Sq=100, causal=True, scale=8.0),
     "many_heads": lambda: Case(B=2, H=16, Hk=8, Sq=65, causal=True, slopes=True),
+    # 512 blocks of 256 rows and more: the row tiles of 8 waves
+    "many_wide_heads": lambda: Case(B=2, H=256, Hk=2, D=128, Sq=300, Sk=97, causal=True, q_start=[-190, -40], kv_len=[97, 60],
+                                    poison=math.nan, fused=False),
+    "many_wide_heads_docs": lambda: Case(B=4, H=128, Hk=4, D=128, Sq=257, causal=True, cap=5.0, slopes=True,
+                                         doc_ids=docs(4, 257, [70, 129, 11], pad=9), poison=math.nan),
     "long": lambda: Case(B=1, H=2, Hk=1, Sq=1100, causal=True, doc_ids=docs(1, 1100, [700, 129, 271])),
 }
 
