@@ -295,6 +295,19 @@ def test_logprobs_special_rows(make, dtype, V):
     check_logprobs(6, V, V, dtype, 12, make=make)
 
 
+def _ones(x, ids):
+    x[:] = 1.0
+
+
+def _rising(x, ids):
+    x[:] = torch.arange(x.shape[1]).float() / 65536  # the best are in the last parts, thousands above any early bound
+
+
+@pytest.mark.parametrize("dtype,make", [(F32, None), (F32, _rising), (BF, _rising), (BF, _ones)])
+def test_logprobs_one_row_of_many_parts(dtype, make):
+    check_logprobs(1, 300001, 300001, dtype, 32, make=make, seed=5)
+
+
 def test_logprobs_nan_and_inf_rows():
     x = randn(4, 3000, dtype=F32)
     x[0, 7] = math.nan
