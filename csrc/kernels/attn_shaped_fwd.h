@@ -178,7 +178,9 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
 // NW ways inside a block and `splits` ways over blocks; each block takes an even share of the keys
 // that its rows see (the lengths are device data). Bound by reading K and V once: K goes from memory
 // straight into operand registers, V through the wave's own LDS (no block barrier in the loop). The
-// waves' (m, l, O) meet in LDS, those of the blocks in shaped_few_join_kernel.
+// waves' (m, l, O) meet in LDS, those of the blocks in shaped_few_join_kernel. B16 H32/8 D128 over caches of up to
+// 16384: 157 us, 5.4 TB/s. B1 H16 D64 Sk 777: 10 us, of which 6 are a launch with no keys at all; its second tile
+// costs as much as the first, a chain of dependent steps and no load (touching the tile's lines early: equal).
 constexpr int FW = 8;  // waves
 template <typename T, int D, typename O>
 __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int splits, float* __restrict__ part) {

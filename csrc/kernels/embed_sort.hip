@@ -11,7 +11,8 @@
 // crosses a chunk border go to a workspace (`part`: a head and a tail row per chunk) and a second
 // launch adds them in chunk order, so a token that fills half the batch is summed by many groups.
 // Without accumulation the rows that no token names are zeroed by extra blocks of the same launch
-// (they find their rows by a search in `keys`), so the table is written once.
+// (they find their rows by a search in `keys`), so the table is written once. Bound by that write and the read
+// of dy: T 8192, W 1024, V 33792 bf16 22 us, 7.0 TB/s; T 65536, W 768, V 131072 100 us and 10 of the join, 4.6 TB/s.
 #include "common.h"
 
 namespace {
@@ -365,7 +366,9 @@ int lanes_per_chunk(int W) {
   }
   return best;
 }
-// positions of a chunk
+// positions of a chunk: short ones give a small batch more groups (333 tokens of width 512: 8 15.4 us, 16 17.1,
+// 64 26.6), long ones cut fewer runs in pieces (65536 tokens of width 768: 8 140 us, 16 127, 32 118, 64 124);
+// 8 and 32 are equal at 4096 and 8192 tokens
 int chunk_of(long long n) { return n <= 4096 ? 8 : 32; }
 template <typename T>
 void emb_sum_launch(const int* keys, const int* perm, int n, int V, int W, const void* dy, long long ldy, float* dword,
@@ -381,6 +384,8 @@ void emb_sum_launch(const int* keys, const int* perm, int n, int V, int W, const
   if (acc) hipLaunchKernelGGL(emb_join_kernel<true>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);
   else hipLaunchKernelGGL(emb_join_kernel<false>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);
 }
+// counting is one launch of T^2 / 2 compares, digits are two launches for each 10 bits of V: 8192 tokens 8 us
+// against 18, 16384 as many as the digits
 constexpr int COUNT_MAX = 16384;
 }  // namespace
 
