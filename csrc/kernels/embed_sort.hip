@@ -12,7 +12,8 @@
 // launch adds them in chunk order, so a token that fills half the batch is summed by many groups.
 // Without accumulation the rows that no token names are zeroed by extra blocks of the same launch
 // (they find their rows by a search in `keys`), so the table is written once. Bound by that write and the read
-// of dy: T 8192, W 1024, V 33792 bf16 22 us, 7.0 TB/s; T 65536, W 768, V 131072 100 us and 10 of the join, 4.6 TB/s.
+// of dy: order and gradient of 8192 tokens, W 1024, V 33792 bf16 45 us (155 MB, 3.5 TB/s; the write alone 21),
+// of 65536 tokens, W 768, V 131072 135 us (503 MB, 3.7 TB/s). Each further launch costs 3 to 6 us of it.
 #include "common.h"
 
 namespace {
@@ -236,36 +237,35 @@ __device__ __forceinline__ int lower_wave(const int* keys, int n, int k) {
 }
 
 // lpc lanes share a chunk (8 columns each, `slabs` groups across a row); blocks from `sumb` on zero
-// the rows without tokens, 64 rows a block. A group loads BATCH rows at once, then adds them in order:
+// the rows without tokens, ZROWS rows a block. A group loads BATCH rows at once, then adds them in order:
 // one row's latency at a time was most of a short batch's 18 us.
 constexpr int BATCH = 8;
+constexpr int ZROWS = 8;  // of a zeroing block: many short blocks (V 33792, W 1024: 8 36.7 us, 16 37.6, 32 38.1, 64 38.8)
 template <typename T, bool ACC>
 __global__ __launch_bounds__(NT) void emb_sum_kernel(const int* __restrict__ keys, const int* __restrict__ perm, int n,
                                                      int V, int W, const T* __restrict__ dy, long long ldy,
                                                      float* __restrict__ dword, float* __restrict__ part, float scale,
                                                      int chunk_len, int lpc, int slabs, int sumb) {
   if ((int)blockIdx.x >= sumb) {
-    __shared__ unsigned has[2];
+    __shared__ unsigned has;
     __shared__ int range[2];
-    const int r0 = ((int)blockIdx.x - sumb) * 64, nr = min(64, V - r0);
-    if (threadIdx.x < 2) has[threadIdx.x] = 0;
+    const int r0 = ((int)blockIdx.x - sumb) * ZROWS, nr = min(ZROWS, V - r0);
+    if (threadIdx.x == 0) has = 0;
     if (threadIdx.x < 128) {
-      const int w = threadIdx.x >> 6, p = lower_wave(keys, n, r0 + w * 64);
+      const int w = threadIdx.x >> 6, p = lower_wave(keys, n, r0 + w * ZROWS);
       if ((threadIdx.x & 63) == 0) range[w] = p;
     }
     __syncthreads();
-    for (int p = range[0] + threadIdx.x; p < range[1]; p += NT) {
-      const int r = keys[p] - r0;
-      if (p == range[0] || keys[p - 1] != keys[p]) atomicOr(&has[r >> 5], 1u << (r & 31));
-    }
+    for (int p = range[0] + threadIdx.x; p < range[1]; p += NT)
+      if (p == range[0] || keys[p - 1] != keys[p]) atomicOr(&has, 1u << (keys[p] - r0));
     __syncthreads();
-    const unsigned m0 = has[0], m1 = has[1];
+    const unsigned named = has;
     const int vpr = W >> 2;
     int r = 0, c = threadIdx.x;
     float* d = dword + (long long)r0 * W;
     while (c >= vpr) { c -= vpr; ++r; }
     for (; r < nr;) {
-      if (!(((r < 32 ? m0 : m1) >> (r & 31)) & 1)) *(f32x4*)(d + (long long)r * W + 4 * c) = f32x4{0.f, 0.f, 0.f, 0.f};
+      if (!((named >> r) & 1)) *(f32x4*)(d + (long long)r * W + 4 * c) = f32x4{0.f, 0.f, 0.f, 0.f};
       c += NT;
       while (c >= vpr) { c -= vpr; ++r; }
     }
@@ -366,16 +366,16 @@ int lanes_per_chunk(int W) {
   }
   return best;
 }
-// positions of a chunk: short ones give a small batch more groups (333 tokens of width 512: 8 15.4 us, 16 17.1,
-// 64 26.6), long ones cut fewer runs in pieces (65536 tokens of width 768: 8 140 us, 16 127, 32 118, 64 124);
-// 8 and 32 are equal at 4096 and 8192 tokens
-int chunk_of(long long n) { return n <= 4096 ? 8 : 32; }
+// positions of a chunk, powers of two that give 512 to 2048 chunks over the middle of the range: short ones give
+// a small batch more groups (accumulating, 8192 tokens of width 1024: 8 17.9 us, 16 19.2, 32 26.5), long ones cut
+// fewer runs in pieces (65536 tokens of width 768: 8 94 us, 16 86, 32 83; 16384 of width 1024: 33.8, 32.5, 38.6)
+int chunk_of(long long n) { return n <= 8192 ? 8 : n <= 32768 ? 16 : 32; }
 template <typename T>
 void emb_sum_launch(const int* keys, const int* perm, int n, int V, int W, const void* dy, long long ldy, float* dword,
                     float* part, float scale, int acc, hipStream_t s) {
   const int lpc = lanes_per_chunk(W), slabs = (W / 8 + lpc - 1) / lpc, cl = chunk_of(n);
   const long long chunks = ((long long)n + cl - 1) / cl;
-  const int sumb = (int)((chunks * slabs * lpc + NT - 1) / NT), zerob = acc ? 0 : (V + 63) / 64;
+  const int sumb = (int)((chunks * slabs * lpc + NT - 1) / NT), zerob = acc ? 0 : (V + ZROWS - 1) / ZROWS;
   if (sumb + zerob == 0) return;
   if (acc) hipLaunchKernelGGL((emb_sum_kernel<T, true>), dim3(sumb), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb);
   else hipLaunchKernelGGL((emb_sum_kernel<T, false>), dim3(sumb + zerob), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb);
