@@ -76,14 +76,31 @@ void check_cols(const torch::Tensor& t, const torch::Tensor& ref, long long off,
   if (write)
     TORCH_CHECK(B == 1 || bs >= (S - 1) * rs + W || (bs >= W && rs >= (B - 1) * bs + W), n, ": tokens overlap");
 }
+// Two column views share no element: disjoint byte ranges, or the same token stride and disjoint columns.
+struct View {
+  const char* at;
+  long long rs, last;  // bytes: token stride, from the first to behind the last element
+  long long w;
+  const char* n;
+};
+View view_of(const torch::Tensor& t, long long off, long long bs, long long rs, long long B, long long S, long long W, const char* n) {
+  return {(const char*)t.data_ptr() + 2 * off, 2 * rs, 2 * ((B - 1) * bs + (S - 1) * rs + W), 2 * W, n};
+}
+void disjoint(const View& a, const View& b) {
+  const bool apart = a.at + a.last <= b.at || b.at + b.last <= a.at;
+  if (apart) return;
+  const View &lo = a.at <= b.at ? a : b, &hi = a.at <= b.at ? b : a;
+  const long long d = a.rs == b.rs && a.rs > 0 ? (hi.at - lo.at) % a.rs : 0;
+  TORCH_CHECK(d >= lo.w && d + hi.w <= a.rs, a.n, " overlaps ", b.n);
+}
 void check_shape(const std::vector<int64_t>& s, double scale, double cap, double p_drop) {
   TORCH_CHECK(s.size() == 6, "attention shape [B,H,Hk,Sq,Sk,D]");
   for (auto v : s) TORCH_CHECK(v >= 1 && v <= 0x7fffffff, "bad attention shape");
   TORCH_CHECK(s[1] % s[2] == 0, "heads must be a multiple of key heads");
   TORCH_CHECK(s[5] == 64 || s[5] == 128, "head dim must be 64 or 128, got ", s[5]);
-  // query rows padded to whole tiles; block counts and row indices are 32-bit
-  TORCH_CHECK((s[3] + 128) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x7ffffff, "sequence too long");
-  TORCH_CHECK(((s[3] + 128) / 32 * (s[1] / s[2]) + s[4] / 64 + 2) * s[0] * s[2] <= 0x7fffffff, "attention grid too large");
+  // query rows padded to whole tiles (of up to 256); block counts and row indices are 32-bit
+  TORCH_CHECK(s[0] * s[1] <= 0x7fffffff && (s[3] + 256) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x7ffffff, "attention shape too large");
+  TORCH_CHECK(((s[3] + 256) / 32 * (s[1] / s[2]) + s[4] / 64 + 2) * s[0] * s[2] <= 0x7fffffff, "attention grid too large");
   TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "scale must be positive, got ", scale);
   TORCH_CHECK(cap >= 0.0 && std::isfinite(cap), "softcap must be >= 0, got ", cap);
   TORCH_CHECK(p_drop >= 0.0 && p_drop < 1.0, "p_drop");
@@ -169,6 +186,15 @@ void shaped_bwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch:
   check_cols(dq, q, dqo, gs[0], gs[1], B, Sq, H * D, true, "dq");
   check_cols(dk, q, dko, gs[2], gs[3], B, Sk, Hk * D, true, "dk");
   check_cols(dv, q, dvo, gs[4], gs[5], B, Sk, Hk * D, true, "dv");
+  const View in[] = {view_of(q, qo, c.st[0], c.st[1], B, Sq, H * D, "q"), view_of(k, ko, c.st[2], c.st[3], B, Sk, Hk * D, "k"),
+                     view_of(v, vo, c.st[4], c.st[5], B, Sk, Hk * D, "v"), view_of(out, 0, c.st[6], c.st[7], B, Sq, H * D, "out"),
+                     view_of(dout, 0, c.st[6], c.st[7], B, Sq, H * D, "dout")};
+  const View gr[] = {view_of(dq, dqo, gs[0], gs[1], B, Sq, H * D, "dq"), view_of(dk, dko, gs[2], gs[3], B, Sk, Hk * D, "dk"),
+                     view_of(dv, dvo, gs[4], gs[5], B, Sk, Hk * D, "dv")};
+  for (int i = 0; i < 3; ++i) {
+    for (const View& x : in) disjoint(gr[i], x);  // every pass reads what the one before it reads
+    for (int j = 0; j < i; ++j) disjoint(gr[i], gr[j]);
+  }
   need_vec(lse, at::kFloat, B * H * Sq, q, "lse");
   const Masks m = masks(kv_len, q_start, prefix, docs, slopes, shape, q);
   torch::Tensor delta = at::empty({2 * B * H * Sq}, lse.options()), ws;
@@ -197,8 +223,8 @@ int check_logits(const torch::Tensor& x, const torch::Tensor& ids, int64_t V, in
   TORCH_CHECK(x.dim() == 2 && (x.size(1) == 1 || x.stride(1) == 1), "logits must be [T, V] with unit column stride");
   TORCH_CHECK(V >= 1 && V <= x.size(1) && x.size(1) <= 0x3fffffff, "logits: ", V, " classes of ", x.size(1), " columns");
   TORCH_CHECK(k >= 0 && k <= tfk_logprobs_kmax() && k <= V, "top_k must be in 0..min(", tfk_logprobs_kmax(), ", V), got ", k);
-  // blocks of a launch: rows times the parts of a row
-  TORCH_CHECK(x.size(0) * ((x.size(1) >> 12) + 1) <= 0x7fffffff, "too many rows");
+  // blocks of a launch: rows times the parts of a row (512 16-byte vectors each, few rows: up to 256 blocks)
+  TORCH_CHECK(x.size(0) <= 0x7fffffff && x.size(0) * ((x.size(1) >> 11) + 1) <= 0x7fffffff, "too many rows");
   need_vec(ids, at::kInt, x.size(0), x, "ids");
   return dt;
 }
@@ -247,7 +273,8 @@ torch::Tensor logprobs_bwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_
 std::tuple<torch::Tensor, torch::Tensor> token_order(torch::Tensor ids, int64_t V) {
   need(ids, at::kInt, "ids");
   const long long T = ids.numel();
-  TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 0x3fffffff, "token_order: V ", V, ", tokens ", T);
+  // (a digit's places are counted over the histograms of all tiles: the square of T / 2048)
+  TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 1 << 24, "token_order: V ", V, ", tokens ", T, " (at most 2^24)");
   const c10::DeviceGuard guard(ids.device());
   torch::Tensor perm = at::empty({T}, ids.options()), keys = at::empty({T}, ids.options()), w;
   const long long ws = tfk_token_order_scratch(T);
@@ -265,15 +292,16 @@ void embedding_bwd_sorted(torch::Tensor perm, torch::Tensor keys, torch::Tensor 
   TORCH_CHECK(dy.dim() == 2 && dword.dim() == 2 && dy.size(1) == dword.size(1), "dy [T, W] and dword [V, W]");
   const long long T = dy.size(0), V = dword.size(0), W = dy.size(1);
   TORCH_CHECK(W >= 8 && W % 8 == 0 && W <= (1 << 20), "embedding width %8, got ", W);
-  TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 0x3fffffff, "embedding_bwd_sorted: V ", V, ", tokens ", T);
-  // blocks of a launch: a group of >= 8 lanes per 32 tokens and 64 columns, and one per 64 rows
-  TORCH_CHECK((T / 32 + 1) * (W / 64 + 1) / 4 + V / 64 + 2 <= 0x7fffffff, "embedding_bwd_sorted: grid too large");
+  TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 1 << 24, "embedding_bwd_sorted: V ", V, ", tokens ", T, " (at most 2^24)");
+  // threads of a launch: W / 8 lanes, in groups of up to 64, for each chunk (2 W words of `part`)
+  const long long words = tfk_emb_sorted_part(T, (int)W);
+  TORCH_CHECK(words / 16 + words / (2 * W) * 64 <= 0x7fffffff, "embedding_bwd_sorted: ", T, " tokens of width ", W, " are too many");
   TORCH_CHECK((dy.size(1) == 1 || dy.stride(1) == 1) && (T <= 1 || (dy.stride(0) >= W && dy.stride(0) % 8 == 0)),
               "dy rows: unit column stride, row stride a multiple of 8");
   need_aligned(dy, 16, "dy"); need_aligned(dword, 16, "dword");
   need_vec(perm, at::kInt, T, dy, "order"); need_vec(keys, at::kInt, T, dy, "order");
   const c10::DeviceGuard guard(dy.device());
-  torch::Tensor part = at::empty({tfk_emb_sorted_part(T, (int)W)}, dword.options());
+  torch::Tensor part = at::empty({words}, dword.options());
   check_rc(tfk_emb_sorted(keys.data_ptr<int>(), perm.data_ptr<int>(), (int)T, (int)V, (int)W, dy.data_ptr(), dt,
                           dy.stride(0), dword.data_ptr<float>(), part.data_ptr<float>(), (float)scale, accumulate ? 1 : 0,
                           stream_of(dy)),

@@ -36,7 +36,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   for (int u = 1; u < NW; ++u) { blo = min(blo, range[0][u]); bhi = max(bhi, range[1][u]); }
   blo = __builtin_amdgcn_readfirstlane(blo);
   bhi = __builtin_amdgcn_readfirstlane(bhi);
-  const int t0 = bhi > 0 ? blo / KT : 0, t1 = (bhi + KT - 1) / KT;
+  // tiles from the first key that a row sees: keys in front of it are not read
+  const int org = bhi > 0 ? blo : 0, t1 = (bhi - org + KT - 1) / KT;
 
   const T* Kb = (const T*)p.k + b * p.k_bs + hk * D;
   const T* Vb = (const T*)p.v + b * p.v_bs + hk * D;
@@ -44,9 +45,10 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   km.init(p.k_rs);
   vm.init(p.v_rs);
   auto issue = [&](int t, int slot) {
-    km.issue(Kb + (long long)t * KT * p.k_rs, p.k_rs, bhi - t * KT, lds + slot * 2 * TB);
-    vm.issue(Vb + (long long)t * KT * p.v_rs, p.v_rs, bhi - t * KT, lds + slot * 2 * TB + TB);
-    if constexpr (DOCS) Dead::issue(mk.docs, 8, 4, p.Sk, t * KT, vm, lds_marks + slot * Dead::WORDS * 4);  // a run's end; 0: in none
+    const int k0 = org + t * KT;
+    km.issue(Kb + k0 * p.k_rs, p.k_rs, bhi - k0, lds + slot * 2 * TB);
+    vm.issue(Vb + k0 * p.v_rs, p.v_rs, bhi - k0, lds + slot * 2 * TB + TB);
+    if constexpr (DOCS) Dead::issue(mk.docs, 8, 4, p.Sk, k0, vm, lds_marks + slot * Dead::WORDS * 4);  // a run's end; 0: in none
   };
   auto landed = [&](int slot) {
     dma_wait();
@@ -60,7 +62,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
     }
     lds_bar();
   };
-  if (t0 < t1) issue(t0, 0);
+  if (t1 > 0) issue(0, 0);
   const T* Qr = (const T*)p.q + b * p.q_bs + qc * p.q_rs + head * D;
   const long long orow = b * p.o_bs + qc * p.o_rs + head * D;
   typename Ty<T>::x8 qf[D / 16], df[D / 16];
@@ -95,13 +97,13 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[db][e] = 0.f;
-  if (t0 < t1) landed(0);
+  if (t1 > 0) landed(0);
   auto step = [&](auto slot_, int t) {
     constexpr int slot = decltype(slot_)::value, KA = slot * 2 * TB, VA = KA + TB;
     if (t + 1 < t1) issue(t + 1, slot ^ 1);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
-      const int k0 = t * KT + 32 * kb;
+      const int k0 = org + t * KT + 32 * kb;
       if (!(k0 < re.uhi && k0 + 32 > re.ulo)) continue;  // wave-uniform
       f32x16 s, dp = ndl;
 #pragma unroll
@@ -151,7 +153,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
     }
     if (t + 1 < t1) landed(slot ^ 1);
   };
-  for (int t = t0; t < t1; t += 2) {
+  for (int t = 0; t < t1; t += 2) {
     step(iconst<0>{}, t);
     if (t + 1 < t1) step(iconst<1>{}, t + 1);
   }
@@ -212,7 +214,8 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   for (int u = 1; u < NW; ++u) { blo = min(blo, range[0][u]); bhi = max(bhi, range[1][u]); }
   blo = __builtin_amdgcn_readfirstlane(blo);
   bhi = __builtin_amdgcn_readfirstlane(bhi);
-  const int t0 = bhi > 0 ? blo / KT : 0, nt = bhi > 0 ? (bhi + KT - 1) / KT - t0 : 0;
+  // tiles from the first query that sees a key of the block (dropout hashes whole quads of queries)
+  const int org = bhi > 0 ? (O::drop ? blo & ~3 : blo) : 0, nt = (bhi - org + KT - 1) / KT;
   // this block's share of the (head, tile) sequence
   const long long all = (long long)nt * p.G;
   const int i0 = (int)(all * split / splits), i1 = (int)(all * (split + 1) / splits);
@@ -222,20 +225,20 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   Dma<D, NW, KT> qm, om;
   qm.init(p.q_rs);
   om.init(p.o_rs);
-  int g_next = i0 / max(nt, 1), t_next = t0 + i0 % max(nt, 1);  // (head, tile) of the next issue
+  int g_next = i0 / max(nt, 1), t_next = i0 % max(nt, 1);  // (head, tile) of the next issue
   // without documents the rows that see nothing are those before position 0 (no prefix)
   const int qa = mk.causal && mk.prefix <= 0 ? -mk.shift : 0;
   auto issue = [&](int slot) {
-    const int q0 = t_next * KT, head = hk * p.G + g_next, rows = min(p.Sq - q0, KT);
+    const int q0 = org + t_next * KT, head = hk * p.G + g_next, rows = min(bhi - q0, KT);
     qm.issue((const T*)p.q + b * p.q_bs + head * D + q0 * p.q_rs, p.q_rs, rows, lds + slot * 2 * TB);
     om.issue((const T*)p.dout + b * p.o_bs + head * D + q0 * p.o_rs, p.o_rs, rows, lds + slot * 2 * TB + TB);
-    // row statistics as they are: lse +inf, delta 0 where a row sees nothing; zeros (with zero rows) past Sq
+    // row statistics as they are: lse +inf, delta 0 where a row sees nothing; zeros (with zero rows) from bhi on
     const float* st = p.delta + ((long long)b * p.H + head) * p.Sq + q0;
     const long long n = (long long)p.B * p.H * p.Sq;
     dma_b32(rows_rsrc(st + (w & 1) * n, 4, rows), lds_stat + (slot * 2 + (w & 1)) * 256, l * 4);
     if constexpr (DOCS) Dead::issue(st, 4, 0, rows, 0, qm, lds_marks + slot * Dead::WORDS * 4);
-    if (++t_next == t0 + nt) {
-      t_next = t0;
+    if (++t_next == nt) {
+      t_next = 0;
       ++g_next;
     }
   };
@@ -279,11 +282,11 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[db][e] = dv[db][e] = 0.f;
-  int g = i0 / max(nt, 1), t = t0 + i0 % max(nt, 1);
-  if (i0 < i1) landed(0, t * KT);
+  int g = i0 / max(nt, 1), t = i0 % max(nt, 1);
+  if (i0 < i1) landed(0, org + t * KT);
   auto step = [&](auto slot_, int i) {
     constexpr int slot = decltype(slot_)::value, QA = slot * 2 * TB, OA = QA + TB;
-    const int q0 = t * KT, head = hk * p.G + g;
+    const int q0 = org + t * KT, head = hk * p.G + g;
     if (i + 1 < i1) issue(slot ^ 1);
     const float slope = O::bias ? p.slopes[head] * LOG2E : 0.f;
     const uint32_t hs = drop ? head_seed(p, b * p.H + head) : 0u;
@@ -374,11 +377,11 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
         }
       }
     }
-    if (++t == t0 + nt) {
-      t = t0;
+    if (++t == nt) {
+      t = 0;
       ++g;
     }
-    if (i + 1 < i1) landed(slot ^ 1, t * KT);
+    if (i + 1 < i1) landed(slot ^ 1, org + t * KT);
   };
   for (int i = i0; i < i1; i += 2) {
     step(iconst<0>{}, i);

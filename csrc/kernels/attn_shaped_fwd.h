@@ -36,7 +36,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
   for (int u = 1; u < NW; ++u) { blo = min(blo, range[0][u]); bhi = max(bhi, range[1][u]); }
   blo = __builtin_amdgcn_readfirstlane(blo);
   bhi = __builtin_amdgcn_readfirstlane(bhi);
-  const int t0 = bhi > 0 ? blo / KT : 0, t1 = (bhi + KT - 1) / KT;
+  // tiles from the first key that a row sees: keys in front of it are not read
+  const int org = bhi > 0 ? blo : 0, t1 = (bhi - org + KT - 1) / KT;
 
   const T* Kb = (const T*)p.k + b * p.k_bs + hk * D;
   const T* Vb = (const T*)p.v + b * p.v_bs + hk * D;
@@ -44,9 +45,10 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
   km.init(p.k_rs);
   vm.init(p.v_rs);
   auto issue = [&](int t, int slot) {
-    km.issue(Kb + (long long)t * KT * p.k_rs, p.k_rs, bhi - t * KT, lds + slot * 2 * TB);
-    vm.issue(Vb + (long long)t * KT * p.v_rs, p.v_rs, bhi - t * KT, lds + slot * 2 * TB + TB);
-    if constexpr (DOCS) Dead::issue(mk.docs, 8, 4, p.Sk, t * KT, vm, lds_marks + slot * Dead::WORDS * 4);  // a run's end; 0: in none
+    const int k0 = org + t * KT;
+    km.issue(Kb + k0 * p.k_rs, p.k_rs, bhi - k0, lds + slot * 2 * TB);
+    vm.issue(Vb + k0 * p.v_rs, p.v_rs, bhi - k0, lds + slot * 2 * TB + TB);
+    if constexpr (DOCS) Dead::issue(mk.docs, 8, 4, p.Sk, k0, vm, lds_marks + slot * Dead::WORDS * 4);  // a run's end; 0: in none
   };
   auto landed = [&](int slot) {
     dma_wait();
@@ -59,7 +61,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
     }
     lds_bar();
   };
-  if (t0 < t1) issue(t0, 0);
+  if (t1 > 0) issue(0, 0);
   const T* Qr = (const T*)p.q + b * p.q_bs + qc * p.q_rs + head * D;
   typename Ty<T>::x8 qf[D / 16];
 #pragma unroll
@@ -77,13 +79,13 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
-  if (t0 < t1) landed(0);
+  if (t1 > 0) landed(0);
   auto step = [&](auto slot_, int t) {
     constexpr int slot = decltype(slot_)::value, KA = slot * 2 * TB, VA = KA + TB;
     if (t + 1 < t1) issue(t + 1, slot ^ 1);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
-      const int k0 = t * KT + 32 * kb;
+      const int k0 = org + t * KT + 32 * kb;
       if (!(k0 < re.uhi && k0 + 32 > re.ulo)) continue;  // wave-uniform
       f32x16 s;
 #pragma unroll
@@ -150,7 +152,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
     }
     if (t + 1 < t1) landed(slot ^ 1);
   };
-  for (int t = t0; t < t1; t += 2) {
+  for (int t = 0; t < t1; t += 2) {
     step(iconst<0>{}, t);
     if (t + 1 < t1) step(iconst<1>{}, t + 1);
   }
@@ -200,9 +202,9 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
   const Span sp = valid ? mk.of<DOCS>(q) : Span{0, 0};
   const bool sees = sp.hi > sp.lo;
   const Reach re(sp, sees);
-  const int a0 = re.uhi > 0 ? re.ulo / KEYS : 0, an = (re.uhi + KEYS - 1) / KEYS - a0, per = (an + splits - 1) / splits;
-  const int t1 = a0 + min(an, (split + 1) * per);
-  int t = a0 + split * per + w;
+  const int org = re.uhi > 0 ? re.ulo : 0, an = (re.uhi - org + KEYS - 1) / KEYS, per = (an + splits - 1) / splits;
+  const int t1 = min(an, (split + 1) * per);
+  int t = split * per + w;
 
   // loads through descriptors that end behind the last key any row sees: keys past it arrive as zeros
   constexpr int NVV = KEYS * D / 8 / 64, RPI = 512 / D;  // 16-byte vectors of V a lane moves, rows of one instruction
@@ -214,9 +216,9 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
   u32x4 kn[KB][D / 16], vn[NVV];
   bool vdead[DOCS ? NVV : 1];
   auto load = [&](int tt) {
-    const int rows = min(re.uhi - tt * KEYS, KEYS);
-    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(Kb + (long long)tt * KEYS * p.k_rs, krs, rows);
-    const __amdgpu_buffer_rsrc_t rv = rows_rsrc(Vb + (long long)tt * KEYS * p.v_rs, vrs, rows);
+    const int k0 = org + tt * KEYS, rows = min(re.uhi - k0, KEYS);
+    const __amdgpu_buffer_rsrc_t rk = rows_rsrc(Kb + k0 * p.k_rs, krs, rows);
+    const __amdgpu_buffer_rsrc_t rv = rows_rsrc(Vb + k0 * p.v_rs, vrs, rows);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -228,7 +230,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
     if constexpr (DOCS) {
 #pragma unroll
       for (int i = 0; i < NVV; ++i) {
-        const int2 d = p.docs[(long long)b * p.Sk + min(tt * KEYS + vrow + i * RPI, p.Sk - 1)];
+        const int2 d = p.docs[(long long)b * p.Sk + min(k0 + vrow + i * RPI, p.Sk - 1)];
         vdead[i] = d.y <= d.x;
       }
     }
@@ -250,7 +252,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
     for (int e = 0; e < 16; ++e) o[db][e] = 0.f;
 
   for (; t < t1; t += FW) {
-    const int k0 = t * KEYS;
+    const int k0 = org + t * KEYS;
     f32x16 s[KB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {

@@ -178,7 +178,7 @@ class TokenOrder:
 def token_order(ids: torch.Tensor, V: int) -> TokenOrder:
     """The order in which embedding_bwd_sorted sums the gradient rows of ids (int32, any shape): one
     order serves every table that is indexed by the same ids. It depends on the ids alone (no host
-    synchronisation, same result from run to run)."""
+    synchronisation, same result from run to run). At most 2^24 tokens."""
     if ids.dtype != torch.int32:
         raise TypeError(f"token_order: ids must be int32, got {ids.dtype}")
     if V < 1:
@@ -336,9 +336,9 @@ class AttnSpec:
     docs        document_spans of the key sequence: a query at position p sees its own document only
                 (positions outside the sequence see nothing)
     kv_len, causal, p_drop and seed as in the plain form (causal compares with p_i). A query that sees
-    no key has output 0, lse +inf and no gradient. Keys that no query of the call can see (beyond kv_len,
-    padding of docs, outside the walked range) may hold anything; a non-finite value in a key that some
-    queries see can reach the others of the same tile. Buffers may be 2-D [B*S, width] or 3-D [B, S', width]
+    no key has output 0, lse +inf and no gradient. Keys that no query of the call sees (beyond kv_len,
+    padding, other documents) may hold anything; a non-finite value in a key that some queries see can
+    reach the others of the same tile. Buffers may be 2-D [B*S, width] or 3-D [B, S', width]
     with S' >= S (a cache with room), rows any multiple of 8 elements apart."""
 
     def __init__(self, B, H, Sq, Sk, q, k, v, kv_len=None, causal=False, p_drop=0.0, seed=0, scale=None, *,

@@ -38,7 +38,7 @@ class Case:
         self.__dict__.update(B=B, H=H, Hk=Hk, D=D, Sq=Sq, Sk=Sk, dtype=dtype, causal=causal, cap=cap, p_drop=p_drop)
         self.kv_len, self.q_start, self.prefix_len = (i32(x) if x is not None else None for x in (kv_len, q_start, prefix_len))
         self.doc_ids = doc_ids
-        self.slopes = torch.tensor([2.0 ** -(1 + h % 7) for h in range(H)]) if slopes else None
+        self.slopes = torch.tensor([slopes * 2.0 ** -(1 + h % 7) for h in range(H)]) if slopes else None
         self.q, self.k, self.v = (randn(B, S, n, D, seed=seed + i, dtype=dtype, scale=scale)
                                   for i, (S, n) in enumerate(((Sq, H), (Sk, Hk), (Sk, Hk))))
         self.dout = randn(B, Sq, H, D, seed=seed + 3, dtype=dtype)
@@ -135,6 +135,10 @@ ATTN = {
     "shared_one": lambda: Case(B=1, H=12, Hk=1, Sq=66, causal=True),
     "dropout": lambda: Case(B=2, H=2, Sq=130, causal=True, cap=7.0, p_drop=0.2, doc_ids=docs(2, 130, [100, 9])),
     "dropout_shared": lambda: Case(B=1, H=4, Hk=2, D=128, Sq=35, Sk=70, p_drop=0.5, fused=False),
+    "dropout_few": lambda: Case(B=2, H=4, Hk=2, Sq=3, Sk=90, causal=True, q_start=[87, 30], p_drop=0.3, fused=False),
+    "slopes_up": lambda: Case(B=2, H=4, Hk=2, Sq=170, causal=True, slopes=-1.0, cap=5.0),
+    "late_chunk_shared_docs": lambda: Case(B=2, H=6, Hk=2, D=128, Sq=130, Sk=330, causal=True, q_start=[199, 70],
+                                           doc_ids=docs(2, 330, [101, 64])),
     "large_scores": lambda: Case(B=1, H=2, Hk=1, Sq=100, causal=True, scale=8.0),
     "many_heads": lambda: Case(B=2, H=16, Hk=8, Sq=65, causal=True, slopes=True),
     # 512 blocks of 256 rows and more: the row tiles of 8 waves
@@ -169,6 +173,25 @@ DECODE = {
 @pytest.mark.parametrize("name", list(DECODE))
 def test_attention_few_queries(name):
     DECODE[name]().check(grads=False)
+
+
+UNSEEN = {
+    "chunk_of_documents": lambda: Case(B=2, H=4, Hk=2, Sq=100, Sk=500, causal=True, q_start=[260, 391], doc_ids=docs(2, 500, [217, 31])),
+    "chunk_both_ways": lambda: Case(B=1, H=2, D=128, Sq=70, Sk=400, q_start=[150], doc_ids=docs(1, 400, [99, 75])),
+    "chunk_dropout": lambda: Case(B=1, H=2, Sq=90, Sk=300, causal=True, q_start=[203], doc_ids=docs(1, 300, [201]), p_drop=0.25),
+    "token_of_documents": lambda: Case(B=2, H=8, Hk=2, Sq=1, Sk=700, causal=True, q_start=[650, 90], doc_ids=docs(2, 700, [333, 77])),
+    "window_of_lengths": lambda: Case(B=3, H=2, Sq=40, Sk=260, causal=True, q_start=[0, 17, 200], kv_len=[260, 33, 210]),
+}
+
+
+@pytest.mark.parametrize("name", list(UNSEEN))
+def test_attention_unseen_keys_hold_anything(name):
+    c = UNSEEN[name]()
+    dead = ~c.ok.any(1)
+    assert dead.any()
+    c.k[dead] = math.nan
+    c.v[dead] = math.inf
+    c.check()
 
 
 def test_attention_few_queries_gradients():
@@ -424,6 +447,10 @@ def test_refusals_before_launch():
     with pytest.raises(RuntimeError, match="overlap"):
         e = torch.empty(1, 8, 128, dtype=BF, device=DEV).expand(2, 8, 128)
         TR.attention_bwd(sp, out, out, lse, (e, 0), (torch.empty_like(q), 0), (torch.empty_like(q), 0))
+    e = torch.empty(16, 256, dtype=BF, device=DEV)
+    for grads in (((q, 0), (e, 0), (e, 128)), ((e, 0), (e, 64), (torch.empty_like(q), 0)), ((e, 0), (e, 128), (out, 0))):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            TR.attention_bwd(sp, out, torch.ones_like(out), lse, *grads)
     with pytest.raises(RuntimeError, match="lse"):
         TR.attention_bwd(sp, out, out, lse[:1], *((torch.empty_like(q), 0) for _ in range(3)))
     with pytest.raises(RuntimeError):
@@ -435,6 +462,65 @@ def test_refusals_before_launch():
 
 
 # ------------------------------------------------------------------------------------- streams, graphs, together
+
+def test_refuses_too_many_tokens():
+    with pytest.raises(RuntimeError, match="2\\^24"):
+        TR.token_order(torch.zeros((1 << 24) + 1, dtype=torch.int32, device=DEV), 5)
+
+
+# ------------------------------------------------------------------------------------- offsets past 32 bits
+
+def test_attention_offsets_past_32_bits():
+    """K and V as columns of tokens 2^22 elements apart, 600 of them: 2.5e9 elements."""
+    for Sq in (1, 70):
+        c = Case(B=1, H=4, Hk=2, Sq=Sq, Sk=600, causal=True, q_start=[600 - Sq], fused=False, cap=4.0)
+        sp = c.spec()
+        want, lse = TR.attention_fwd(sp)
+        wide = torch.empty(1, 600, 1 << 22, dtype=BF, device=DEV)
+        for i, x in enumerate((c.k, c.v)):
+            wide[0, :, 128 * i:128 * i + 128] = x[0].reshape(600, 128).to(DEV)
+        sp2 = TR.AttnSpec(1, 4, Sq, 600, sp.q, (wide, 0), (wide, 128), causal=True, kv_heads=2, q_start=sp.q_start, softcap=4.0)
+        got, lse2 = TR.attention_fwd(sp2)
+        assert torch.equal(got, want) and torch.equal(lse, lse2)
+        dout = c.dout.reshape(Sq, -1).to(DEV)
+        g = [torch.empty(n, w, dtype=BF, device=DEV) for n, w in ((Sq, 256), (600, 128), (600, 128))]
+        TR.attention_bwd(sp, want, dout, lse, *((x, 0) for x in g))
+        dq2 = torch.empty_like(g[0])
+        TR.attention_bwd(sp2, got, dout, lse2, (dq2, 0), (wide, 256), (wide, 384))
+        assert torch.equal(dq2, g[0])
+        assert torch.equal(wide[0, :, 256:384], g[1]) and torch.equal(wide[0, :, 384:512], g[2])
+        del wide
+
+
+def test_logprobs_offsets_past_32_bits():
+    T, V = 66000, 33001
+    x = torch.empty(T, V, dtype=BF, device=DEV)
+    rows = [0, 1, T - 2, T - 1]  # rows far apart, with the same content at both ends
+    part = randn(4, V, seed=3).to(DEV)
+    x.zero_()
+    x[rows] = part
+    ids = torch.zeros(T, dtype=torch.int32, device=DEV)
+    few = i32([5, 6, 7, 8]).to(DEV)
+    ids[rows] = few
+    r, w = L.token_logprobs(x, ids, top_k=4), L.token_logprobs(part, few, top_k=4)
+    for n in ("logp", "lse", "entropy", "top_logp"):
+        assert torch.allclose(getattr(r, n)[rows], getattr(w, n), rtol=1e-5, atol=1e-5), n
+    assert torch.equal(r.top_ids[rows], w.top_ids)
+    d = L.token_logprobs_bwd(x, ids, r, dlogp=torch.ones(T, device=DEV))
+    dw = L.token_logprobs_bwd(part, few, w, dlogp=torch.ones(4, device=DEV))
+    assert torch.allclose(d[rows].float(), dw.float(), rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_sorted_embedding_offsets_past_32_bits():
+    V, W = 270000, 8192
+    ids = i32([0, V - 1, 3, V - 1]).to(DEV)
+    dy = randn(4, W, seed=1).to(DEV)
+    dw = torch.full((V, W), math.nan, device=DEV)
+    TR.embedding_bwd_sorted(TR.token_order(ids, V), dy, dw, accumulate=False)
+    f = dy.float()
+    assert torch.equal(dw[0], f[0]) and torch.equal(dw[3], f[2]) and torch.equal(dw[V - 1], f[1] + f[3])
+    assert not dw[1:3].any() and not dw[4:V - 1].any()
+
 
 def _step(ids, docs_ids, table, wqkv, targets, H, Hk, D):
     """One training step of a single attention block on packed documents, with the operators as a user
