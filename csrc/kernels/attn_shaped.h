@@ -276,6 +276,15 @@ __device__ __forceinline__ typename Ty<T>::x8 pack8(const f32x16& a, int half) {
   return r;
 }
 
+// what pack8 leaves of a half: a - pack8(a)
+template <typename T>
+__device__ __forceinline__ typename Ty<T>::x8 pack8_rest(const f32x16& a, int half, typename Ty<T>::x8 hi) {
+  typename Ty<T>::x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)(a[8 * half + e] - (float)hi[e]);
+  return r;
+}
+
 // A tile of KT rows of D elements from memory straight into the LDS (buffer loads with LDS destination, 16
 // bytes a lane): instruction i of wave w fills rows (i NW + w) RPI .. + RPI - 1, the swizzle is in the
 // lanes' source addresses. Rows from `rows` on lie past the descriptor's end and arrive as zeros.

@@ -5,7 +5,14 @@
 
 namespace {
 // ------------------------------------------------------------------------------- dQ pass
-// same rows and tiles as the forward; also writes lse in log2 units (shifted, Score) and -rowsum(dO * O)
+// same rows and tiles as the forward; also writes lse in log2 units (shifted, Score) and -delta.
+// Precision: delta = sum P dP is taken as dO.O here, off by O's rounding. Beside the roundings of dS and of the
+// gradients this weighs as much as they do where a row's softmax rests on few keys, 1 / n_eff of it else (974 keys
+// under a slope of 1/2 gave 1.7 times the error of a float32 backward, 372 without one 1.48). So where a row of the
+// wave sees at most FEW keys, or its slope leaves it about as many, sum P (dP - delta) over the row, which is that
+// error, corrects the delta of the dK/dV pass, and dQ, where it stays, takes dS into its product as two 16-bit
+// terms. (Everywhere: B1 H16/4 S8192 D128 dQ 417 -> 580 us, B4 H16 S2048 D64 documents 35 -> 41.)
+constexpr int FEW = 128;
 template <typename T, int D, int NW, typename O>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Shaped p) {
   constexpr bool DOCS = O::docs;
@@ -79,10 +86,6 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   const long long srow_i = ((long long)b * p.H + head) * p.Sq + qc;
   const Score<O> sc(p);
   const float lse2 = sees ? fmaf(p.lse[srow_i], LOG2E, -sc.base) : INFINITY;
-  if (valid && h == 0) {  // for the dK/dV pass
-    p.delta[srow_i] = lse2;
-    p.delta[(long long)p.B * p.H * p.Sq + srow_i] = -dlt;
-  }
   const float slope = O::bias ? p.slopes[head] * LOG2E : 0.f;
   const int pos = q + mk.shift;
   const int thr = drop_thr(p.p_drop);
@@ -90,6 +93,8 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   const float keep = drop ? 256.f / (float)(256 - thr) : 1.f;
   const uint32_t hs = drop ? head_seed(p, b * p.H + head) : 0u;
   const int qg = (q >> 2) * p.Sk;
+  const bool two = __any(sees && (sp.hi - sp.lo <= FEW || (O::bias && slope * FEW >= 2.f * LOG2E)));  // e^-2 at FEW
+  float rest = 0.f;  // this lane's half of sum P (dP - delta)
   f32x16 acc[D / 32], ndl;  // -delta in every slot: dP - delta is the product's start
 #pragma unroll
   for (int e = 0; e < 16; ++e) ndl[e] = -dlt;
@@ -121,34 +126,36 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
           for (int u = 0; u < 4; ++u) dp[e + u] = fmaf((kp & (1u << u)) ? dp[e + u] + dlt : 0.f, keep, -dlt);
         }
       }
-      if (O::bias) {
-        const float d0 = (float)(pos - k0 - 4 * h);
+      // P (dP - delta) in s; capped: d tanh / 4 in dp
+      const float d0 = O::bias ? (float)(pos - k0 - 4 * h) : 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float x = s[e] * sc.mult;
-          if (O::cap) {
-            const float r_ = sc.r(s[e]);
-            x = sc.c2l * r_;
-            dp[e] *= fmaf(-r_, r_, r_);
-          }
-          s[e] = ex2(fmaf(-slope, fabsf(d0 - (float)srow(e)), x - lse2)) * dp[e];
-        }
-      } else if (O::cap) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float r_ = sc.r(s[e]);
-          s[e] = ex2(fmaf(r_, sc.c2l, -lse2)) * (fmaf(-r_, r_, r_) * dp[e]);
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = ex2(fmaf(s[e], sc.mult, -lse2)) * dp[e];
+      for (int e = 0; e < 16; ++e) {
+        const float r_ = O::cap ? sc.r(s[e]) : 0.f;
+        const float x = O::cap ? fmaf(r_, sc.c2l, -lse2) : fmaf(s[e], sc.mult, -lse2);
+        s[e] = ex2(O::bias ? fmaf(-slope, fabsf(d0 - (float)srow(e)), x) : x) * dp[e];
+        if (O::cap) dp[e] = fmaf(-r_, r_, r_);
       }
       if (!(k0 >= re.ilo && k0 + 32 <= re.ihi)) mask_slots(s, (unsigned)(k0 + 4 * h - sp.lo), (unsigned)(sp.hi - sp.lo), 0.f);
+      if (two) {
+        float a = s[0] + s[1], b_ = s[2] + s[3];
+#pragma unroll
+        for (int e = 4; e < 16; e += 4) { a += s[e] + s[e + 1]; b_ += s[e + 2] + s[e + 3]; }
+        rest += a + b_;
+      }
+      if (O::cap) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] *= dp[e];
+      }
 #pragma unroll
       for (int kc = 0; kc < 2; ++kc) {
-        const typename Ty<T>::x8 sf = pack8<T>(s, kc);
+        const typename Ty<T>::x8 hi = pack8<T>(s, kc);
 #pragma unroll
-        for (int db = 0; db < D / 32; ++db) acc[db] = Ty<T>::mfma(frag_tr<T, D>(smem, KA, fo, 2 * kb + kc, db), sf, acc[db]);
+        for (int db = 0; db < D / 32; ++db) acc[db] = Ty<T>::mfma(frag_tr<T, D>(smem, KA, fo, 2 * kb + kc, db), hi, acc[db]);
+        if (two) {
+          const typename Ty<T>::x8 lo = pack8_rest<T>(s, kc, hi);
+#pragma unroll
+          for (int db = 0; db < D / 32; ++db) acc[db] = Ty<T>::mfma(frag_tr<T, D>(smem, KA, fo, 2 * kb + kc, db), lo, acc[db]);
+        }
       }
     }
     if (t + 1 < t1) landed(slot ^ 1);
@@ -156,6 +163,11 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   for (int t = 0; t < t1; t += 2) {
     step(iconst<0>{}, t);
     if (t + 1 < t1) step(iconst<1>{}, t + 1);
+  }
+  rest = xor_sum<32>(rest);
+  if (valid && h == 0) {  // for the dK/dV pass
+    p.delta[srow_i] = lse2;
+    p.delta[(long long)p.B * p.H * p.Sq + srow_i] = -(dlt + rest);
   }
   if (valid) {
     const float f = O::cap ? 4.f * p.scale : p.scale;

@@ -223,6 +223,29 @@ def test_attention_matches_plain_form():
     assert torch.allclose(a[1], b[1], atol=1e-4)
 
 
+PRECISE = {
+    "short_documents": lambda dt: Case(B=2, H=4, Hk=2, Sq=256, causal=True, dtype=dt, doc_ids=docs(2, 256, [9, 17, 40])),
+    "steep_slopes": lambda dt: Case(B=1, H=1, D=128, Sq=400, causal=True, dtype=dt, slopes=1.0),
+    "first_keys": lambda dt: Case(B=4, H=4, Sq=100, causal=True, cap=20.0, dtype=dt),
+}
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("name", list(PRECISE))
+def test_attention_gradients_have_two_roundings(name, dtype):
+    """Rows that rest on few keys: the relative 2-norm of each gradient's error is at most that of two roundings
+    of its type, sqrt(2) times the error of the exact gradient rounded once (and 6% for the rest)."""
+    c = PRECISE[name](dtype)
+    r, sp = c.oracle(), c.spec()
+    out, lse = TR.attention_fwd(sp)
+    g = [torch.empty(c.B * S, n * c.D, dtype=dtype, device=DEV) for S, n in ((c.Sq, c.H), (c.Sk, c.Hk), (c.Sk, c.Hk))]
+    TR.attention_bwd(sp, out, c.dout.reshape(c.B * c.Sq, -1).to(DEV), lse, *((x, 0) for x in g))
+    for n, x in zip(("dq", "dk", "dv"), g):
+        w = r[n]
+        once = (w.to(dtype).double() - w).norm()
+        assert (x.view(w.shape).double().cpu() - w).norm() <= 1.5 * once, n
+
+
 def test_attention_repeats_bitwise():
     c = Case(B=2, H=4, Hk=2, Sq=200, causal=True, cap=6.0, doc_ids=docs(2, 200, [90, 30]))
     res = []
