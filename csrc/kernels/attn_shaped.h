@@ -25,11 +25,11 @@
 // is read with the same row order: two ds_read_b64_tr_b16 of rows 4h.. and 8 + 4h.. of each 16.
 // LDS rows are D elements, their 16-byte chunks XOR-swizzled (swz): conflict-free for both reads.
 //
-// Bound by arithmetic: an element costs 2 D (dQ: 3 D, dK/dV: 4 D) matrix flops and 9 to 20 vector instructions
+// Bound by arithmetic: an element costs 4 D (dQ: 6 D, dK/dV: 8 D) matrix flops and 9 to 20 vector instructions
 // with one or two exponentials, and the two units overlap only between the waves of a SIMD (vector unit busy
-// 60 to 66%, matrix unit 37 to 48%). B1 H16/4 S8192 D128 bf16, causal, capped: forward 346 us (795 TFLOP/s),
-// dQ 417 us (990), dK/dV 564 us (975) and 24 us of its join. B4 H16 S2048 D64 in documents of about 512: 28, 35
-// and 49 us, half of them the exponentials and masks of tiles that a document fills in part.
+// 60 to 66%, matrix unit 37 to 48%). B1 H16/4 S8192 D128 bf16, causal, capped: forward 358 us (770 TFLOP/s),
+// dQ 453 us (910), dK/dV 576 us (955) and 24 us of its join. B4 H16 S2048 D64 in documents of about 512: 29, 41
+// and 53 us, half of them the exponentials and masks of tiles that a document fills in part.
 #pragma once
 #include <algorithm>
 #include "common.h"
