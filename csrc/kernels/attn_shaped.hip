@@ -14,10 +14,10 @@ int tfk_shaped_dkv_f16(const void*, float*, hipStream_t, int);
 
 namespace {
 // out[b][i] = [first, end) of the run of equal ids around position i; (0, 0) where the id is negative.
-// One block per row: each thread scans a segment, the block scans the segments' borders.
+// One block per row: each thread scans a segment, waves and then the block the segments' borders.
 constexpr int DT = 1024;
 __global__ __launch_bounds__(DT) void doc_spans_kernel(const int* __restrict__ ids, int S, int2* __restrict__ out) {
-  __shared__ int first[DT], next[DT];
+  __shared__ int first[DT / 64], next[DT / 64];
   const int* x = ids + (long long)blockIdx.x * S;
   int2* y = out + (long long)blockIdx.x * S;
   const int per = (S + DT - 1) / DT, i0 = min(S, (int)threadIdx.x * per), i1 = min(S, i0 + per);
@@ -27,23 +27,28 @@ __global__ __launch_bounds__(DT) void doc_spans_kernel(const int* __restrict__ i
       if (f < 0) n = i;
       f = i;
     }
-  first[threadIdx.x] = f;
-  next[threadIdx.x] = n;
-  __syncthreads();
-  for (int o = 1; o < DT; o <<= 1) {  // running max of the last borders, running min of the first ones behind
-    const int a = (int)threadIdx.x >= o ? first[threadIdx.x - o] : -1;
-    const int b = (int)threadIdx.x + o < DT ? next[threadIdx.x + o] : S;
-    __syncthreads();
-    first[threadIdx.x] = max(first[threadIdx.x], a);
-    next[threadIdx.x] = min(next[threadIdx.x], b);
-    __syncthreads();
+  // running max of the last borders in front of this segment, running min of the first ones behind it
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int a = __shfl_up(f, o, 64), b = __shfl_down(n, o, 64);
+    if (l >= o) f = max(f, a);
+    if (l + o < 64) n = min(n, b);
   }
-  int cur = threadIdx.x > 0 ? first[threadIdx.x - 1] : 0;
+  if (l == 63) first[w] = f;
+  if (l == 0) next[w] = n;
+  __syncthreads();
+  int cur = __shfl_up(f, 1, 64), end = __shfl_down(n, 1, 64);
+  if (l == 0) cur = -1;
+  if (l == 63) end = S;
+  for (int u = 0; u < DT / 64; ++u) {
+    if (u < w) cur = max(cur, first[u]);
+    if (u > w) end = min(end, next[u]);
+  }
   for (int i = i0; i < i1; ++i) {
     if (i == 0 || x[i] != x[i - 1]) cur = i;
     y[i].x = x[i] < 0 ? 0 : cur;
   }
-  int end = threadIdx.x + 1 < DT ? next[threadIdx.x + 1] : S;
   for (int i = i1 - 1; i >= i0; --i) {
     y[i].y = x[i] < 0 ? 0 : end;
     if (i == 0 || x[i] != x[i - 1]) end = i;
