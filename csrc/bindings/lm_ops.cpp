@@ -273,7 +273,7 @@ torch::Tensor logprobs_bwd(torch::Tensor x, torch::Tensor ids, int64_t V, int64_
 std::tuple<torch::Tensor, torch::Tensor> token_order(torch::Tensor ids, int64_t V) {
   need(ids, at::kInt, "ids");
   const long long T = ids.numel();
-  // (a digit's places are counted over the histograms of all tiles: the square of T / 2048)
+  // (a digit's places are counted over the histograms of all tiles: the square of T / 4096)
   TORCH_CHECK(V >= 1 && V < 0x7fffffff && T <= 1 << 24, "token_order: V ", V, ", tokens ", T, " (at most 2^24)");
   const c10::DeviceGuard guard(ids.device());
   torch::Tensor perm = at::empty({T}, ids.options()), keys = at::empty({T}, ids.options()), w;

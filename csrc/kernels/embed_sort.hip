@@ -85,14 +85,18 @@ __global__ __launch_bounds__(1024) void order_count_kernel(const int* __restrict
 // One pass of a stable least-significant-digit sort: histogram of each tile, then every tile finds
 // its digits' places from all histograms and writes its items in order.
 constexpr int RT = 512, RW = RT / 64;  // threads, waves of a sorting block
-constexpr int RTILE = 2048;            // items of a tile (each wave: 256 consecutive ones)
 constexpr int RB_MAX = 10;             // digit bits
+// items of a tile (each wave: consecutive ones): small tiles for more blocks, large ones because each block reads
+// the histograms of all tiles (65536 items of 18 bits: 1024 19.1 us, 2048 21.0, 4096 27.7; 2^20 of 16 bits: 108, 60,
+// 48; 2^22 of 18 bits: 2309, 664, 262)
+constexpr int RTILE_FEW = 1024, RTILE_MANY = 4096;
+int radix_tile(long long T) { return T <= 131072 ? RTILE_FEW : RTILE_MANY; }
 
 template <bool FIRST>
 __device__ __forceinline__ int radix_key(const int* src, long long i, int V) {
   return FIRST ? key_of(src[i], V) : src[i];
 }
-template <bool FIRST>
+template <bool FIRST, int RTILE>
 __global__ __launch_bounds__(RT) void radix_hist_kernel(const int* __restrict__ src, int T, int V, int shift, int bits,
                                                         int* __restrict__ hist) {
   __shared__ int h[1 << RB_MAX];
@@ -104,7 +108,7 @@ __global__ __launch_bounds__(RT) void radix_hist_kernel(const int* __restrict__ 
   __syncthreads();
   for (int d = threadIdx.x; d < nd; d += RT) hist[(long long)blockIdx.x * nd + d] = h[d];
 }
-template <bool FIRST>
+template <bool FIRST, int RTILE>
 __global__ __launch_bounds__(RT) void radix_place_kernel(const int* __restrict__ src, const int* __restrict__ psrc, int T,
                                                          int V, int shift, int bits, const int* __restrict__ hist,
                                                          int* __restrict__ dst, int* __restrict__ pdst) {
@@ -186,6 +190,12 @@ __global__ __launch_bounds__(RT) void radix_place_kernel(const int* __restrict__
       pdst[p] = v[u];
     }
   }
+}
+
+template <bool FIRST, int RTILE>
+void radix_pass(const int* ks, const int* ps, int T, int V, int shift, int bits, int nb, int* hist, int* kd, int* pd, hipStream_t s) {
+  hipLaunchKernelGGL((radix_hist_kernel<FIRST, RTILE>), dim3(nb), dim3(RT), 0, s, ks, T, V, shift, bits, hist);
+  hipLaunchKernelGGL((radix_place_kernel<FIRST, RTILE>), dim3(nb), dim3(RT), 0, s, ks, ps, T, V, shift, bits, hist, kd, pd);
 }
 
 // ------------------------------------------------------------------------------- gradient
@@ -384,16 +394,16 @@ void emb_sum_launch(const int* keys, const int* perm, int n, int V, int W, const
   if (acc) hipLaunchKernelGGL(emb_join_kernel<true>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);
   else hipLaunchKernelGGL(emb_join_kernel<false>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);
 }
-// counting is one launch of T^2 / 2 compares, digits are two launches for each 10 bits of V: 8192 tokens 8 us
-// against 18, 16384 as many as the digits
-constexpr int COUNT_MAX = 16384;
+// counting is one launch of T^2 compares (8192 tokens, a block on each CU: 8 us), digits are two launches for each 10
+// bits of V: 12288 tokens 17 us against 20 for 12289 by digits, 16384 22 against 15
+constexpr int COUNT_MAX = 12288;
 }  // namespace
 
 extern "C" {
 // int32 words of scratch that tfk_token_order needs
 long long tfk_token_order_scratch(long long T) {
   if (T <= COUNT_MAX) return 0;
-  const long long nb = (T + RTILE - 1) / RTILE;
+  const long long tile = radix_tile(T), nb = (T + tile - 1) / tile;
   return nb * (1 << RB_MAX) + 2 * T;
 }
 int tfk_token_order(const int* ids, int T, int V, int* perm, int* keys, int* scratch, hipStream_t s) {
@@ -405,19 +415,19 @@ int tfk_token_order(const int* ids, int T, int V, int* perm, int* keys, int* scr
   int total = 1;
   while (total < 31 && (V >> total)) ++total;  // bits of the largest key, V
   const int passes = (total + RB_MAX - 1) / RB_MAX, bits = (total + passes - 1) / passes;
-  const int nb = (T + RTILE - 1) / RTILE;
+  const int tile = radix_tile(T), nb = (T + tile - 1) / tile;
   int *hist = scratch, *k2 = scratch + (long long)nb * (1 << RB_MAX), *p2 = k2 + T;
   const int *ks = ids, *ps = nullptr;
   for (int p = 0; p < passes; ++p) {
     // the last pass writes keys / perm; the passes before it alternate
     const bool fin = ((passes - 1 - p) & 1) == 0;
     int *kd = fin ? keys : k2, *pd = fin ? perm : p2;
-    if (p == 0) {
-      hipLaunchKernelGGL(radix_hist_kernel<true>, dim3(nb), dim3(RT), 0, s, ks, T, V, 0, bits, hist);
-      hipLaunchKernelGGL(radix_place_kernel<true>, dim3(nb), dim3(RT), 0, s, ks, ps, T, V, 0, bits, hist, kd, pd);
+    if (tile == RTILE_FEW) {
+      if (p == 0) radix_pass<true, RTILE_FEW>(ks, ps, T, V, 0, bits, nb, hist, kd, pd, s);
+      else radix_pass<false, RTILE_FEW>(ks, ps, T, V, p * bits, bits, nb, hist, kd, pd, s);
     } else {
-      hipLaunchKernelGGL(radix_hist_kernel<false>, dim3(nb), dim3(RT), 0, s, ks, T, V, p * bits, bits, hist);
-      hipLaunchKernelGGL(radix_place_kernel<false>, dim3(nb), dim3(RT), 0, s, ks, ps, T, V, p * bits, bits, hist, kd, pd);
+      if (p == 0) radix_pass<true, RTILE_MANY>(ks, ps, T, V, 0, bits, nb, hist, kd, pd, s);
+      else radix_pass<false, RTILE_MANY>(ks, ps, T, V, p * bits, bits, nb, hist, kd, pd, s);
     }
     ks = kd;
     ps = pd;

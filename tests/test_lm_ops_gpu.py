@@ -406,7 +406,7 @@ def zipf(T, V, seed=0):
 @pytest.mark.parametrize("T,V,W,dtype,scale,acc", [
     (1, 1, 8, BF, 1.0, True), (1, 5, 64, F32, 2.0, False), (2, 3, 72, HF, 1.0, False), (31, 4, 128, BF, 1.0, True),
     (33, 100, 200, BF, 5.0, False), (64, 1, 64, BF, 1.0, False), (333, 4099, 512, BF, 22.6, False), (1000, 7, 768, F32, 1.0, True),
-    (8192, 3000, 96, BF, 1.0, False), (16384, 500, 64, HF, 1.0, True), (16385, 500, 64, BF, 1.0, False),
+    (8192, 3000, 96, BF, 1.0, False), (12288, 900, 64, BF, 1.0, False), (12289, 900, 64, F32, 1.0, True), (16384, 500, 64, HF, 1.0, True), (16385, 500, 64, BF, 1.0, False),
     (20000, 40, 8, BF, 1.0, False), (40000, 131072, 16, BF, 1.0, True), (33000, 2_000_000, 8, F32, 1.0, True),
 ])
 def test_sorted_embedding(T, V, W, dtype, scale, acc):
@@ -485,6 +485,13 @@ def test_refusals_before_launch():
 
 
 # ------------------------------------------------------------------------------------- streams, graphs, together
+
+@pytest.mark.parametrize("T,V", [(131072, 70000), (131073, 70000), (300001, 9)])
+def test_token_order_of_many_tokens(T, V):
+    ids = torch.randint(-3, V + 3, (T,), generator=torch.Generator().manual_seed(T), dtype=torch.int32)
+    a, b = TR.token_order(ids.to(DEV), V), TR.token_order(ids, V)
+    assert torch.equal(a.perm.cpu(), b.perm) and torch.equal(a.keys.cpu(), b.keys)
+
 
 def test_refuses_too_many_tokens():
     with pytest.raises(RuntimeError, match="2\\^24"):
