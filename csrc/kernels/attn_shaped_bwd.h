@@ -451,10 +451,11 @@ __global__ __launch_bounds__(256) void shaped_dkv_join_kernel(Shaped p, int spli
   *(typename Ty<T>::x4*)d = v;
 }
 
-// shares of a key tile's queries: about 2 blocks for each of 256 CUs (4 cost
-// B1 H16/4 S8192 D128 50 us more, the join's f32 parts), none below 1024 queries
+// shares of a key tile's queries: about 2 blocks for each of 256 CUs (4 cost B1 H16/4 S8192 D128 50 us more, the
+// join's f32 parts), none below 256 queries (forward and backward of B2 H4/1 S1459 D128: 1024 179 us, 512 148,
+// 256 138; B4 H8/2 S600 D128: 117, 85, 77)
 int dkv_splits(long long blocks, int G, int Sq) {
-  return (int)std::max(1ll, std::min((512 + blocks - 1) / blocks, (long long)G * ((Sq + 63) / 64) / 16));
+  return (int)std::max(1ll, std::min((512 + blocks - 1) / blocks, (long long)G * ((Sq + 63) / 64) / 4));
 }
 template <typename T, int D>
 int launch_dq(Shaped p, hipStream_t s) {
