@@ -357,17 +357,18 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
     __syncthreads();
   }
   if (w != 0 || !valid) return;
-  if (splits > 1) {
+  if (splits > 1) {  // (a row that sees nothing went through tiles that its neighbours see whole: no part of it stays)
     float* P = part + ((long long)blockIdx.x * R + r) * D + 4 * h;
+    const f32x4 none = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
       for (int e = 0; e < 16; e += 4)
-        *(f32x4*)(P + db * 32 + srow(e)) = f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]};
+        *(f32x4*)(P + db * 32 + srow(e)) = sees ? f32x4{o[db][e], o[db][e + 1], o[db][e + 2], o[db][e + 3]} : none;
     if (h == 0) {
       float* S = part + (long long)gridDim.x * R * D + ((long long)blockIdx.x * R + r) * 2;
-      S[0] = M;
-      S[1] = L;
+      S[0] = sees ? M : -INFINITY;
+      S[1] = sees ? L : 0.f;
     }
     return;
   }

@@ -1,0 +1,52 @@
+"""Calls of the language-model operators at their edges: rows that see nothing in a cache divided over blocks, small and
+large gradients in half precision, large score caps, lone tokens with odd strides, ids and limits."""
+import math
+
+import pytest
+import torch
+
+import lm_oracle as O
+from tensorflow_k8s_amd.ops import loss as L
+from tensorflow_k8s_amd.ops import transformer as TR
+from test_lm_ops_gpu import BF, DEV, F32, HF, Case, dev, docs, i32, randn, zipf
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------- few rows over a divided cache
+
+def _ids(S, *rows):
+    """Document ids of rows given as runs (id, length), cut or padded (-1) to S."""
+    return i32([([d for d, n in row for _ in range(n)] + [-1] * S)[:S] for row in rows])
+
+
+# every cache is 1024 keys or longer: its keys are divided over blocks
+DIVIDED = {
+    # the first queries see a whole run, the others stand in the padding or behind the last key
+    "padded_tail": lambda: Case(B=2, H=4, Hk=2, Sq=8, Sk=1024, q_start=[996, 1020], doc_ids=_ids(1024, [(0, 1000)], [(0, 1024)])),
+    "padded_tail_causal": lambda: Case(B=2, H=4, Hk=2, D=128, Sq=8, Sk=1024, causal=True, q_start=[996, 1020],
+                                       doc_ids=_ids(1024, [(0, 1000)], [(3, 1024)])),
+    "padded_tail_cap": lambda: Case(B=1, H=2, Hk=1, Sq=8, Sk=1500, causal=True, cap=5.0, q_start=[1196], doc_ids=_ids(1500, [(0, 1200)])),
+    "padded_tail_bias_f16": lambda: Case(B=1, H=4, Hk=1, D=128, Sq=5, Sk=2100, dtype=HF, slopes=True, cap=9.0, q_start=[2097],
+                                         doc_ids=_ids(2100, [(0, 300), (1, 1800)])),
+    "padded_inside": lambda: Case(B=1, H=2, Hk=2, Sq=30, Sk=1600, causal=True, q_start=[1290], doc_ids=_ids(1600, [(0, 1300), (-1, 9), (1, 291)])),
+    "before_the_first_key": lambda: Case(B=2, H=4, Hk=2, Sq=6, Sk=1100, causal=True, q_start=[-3, 1090], slopes=True),
+    "all_padding": lambda: Case(B=2, H=2, Hk=1, Sq=3, Sk=1030, q_start=[500, 9], doc_ids=_ids(1030, [(-1, 1030)], [(0, 1030)])),
+    # shares that lie outside some rows' keys
+    "documents": lambda: Case(B=2, H=4, Hk=2, D=128, Sq=8, Sk=2500, causal=True, q_start=[1596, 700],
+                              doc_ids=_ids(2500, [(0, 900), (1, 700), (2, 900)], [(0, 704), (1, 1700)])),
+    "prefix": lambda: Case(B=3, H=4, Hk=2, Sq=4, Sk=1700, causal=True, q_start=[10, 0, 1696], prefix_len=[1300, 0, 90]),
+    "prefix_kv_len": lambda: Case(B=3, H=2, Hk=1, D=128, Sq=4, Sk=1700, causal=True, q_start=[10, 5, 900], prefix_len=[1300, 40, 90], kv_len=[1200, 0, 901]),
+    "lengths_both_ways": lambda: Case(B=4, H=8, Hk=2, Sq=3, Sk=1300, kv_len=[0, 1300, 1, 700], slopes=True, cap=20.0),
+    "slopes_cap_f16": lambda: Case(B=2, H=4, Hk=4, D=128, Sq=1, Sk=1900, dtype=HF, slopes=True, cap=15.0, kv_len=[1900, 650]),
+}
+
+
+@pytest.mark.parametrize("name", list(DIVIDED))
+def test_attention_divided_cache(name):
+    c = DIVIDED[name]()
+    c.fused = False
+    dead_q, dead_k = ~c.ok.any(2), ~c.ok.any(1)
+    c.q[dead_q] = math.nan  # rows and keys that no pair uses hold anything
+    c.k[dead_k], c.v[dead_k] = math.nan, math.inf
+    c.check(grads=False)  # (0 and lse +inf where a row sees nothing)
