@@ -409,14 +409,8 @@ def _shaped_view(buf, col, B, S, heads, D):
 def _shaped_ref(sp, q, k, v):
     """f32 reference of shaped attention on q [B,Sq,H,D], k, v [B,Sk,Hk,D] -> (out, lse)."""
     B, H, Sq, Sk, G = sp.B, sp.H, sp.Sq, sp.Sk, sp.H // sp.kv_heads
-    k, v = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
-    s = torch.einsum("bqhd,bkhd->bhqk", q, k) * sp.scale
-    if sp.softcap:
-        s = sp.softcap * torch.tanh(s / sp.softcap)
     j = torch.arange(Sk)
     p = torch.arange(Sq)[None, :] + (sp.q_start.long()[:, None] if sp.q_start is not None else torch.zeros(B, 1, dtype=torch.long))
-    if sp.slopes is not None:
-        s = s - sp.slopes[None, :, None, None] * (p[:, :, None] - j).abs()[:, None]
     ok = torch.ones(B, Sq, Sk, dtype=torch.bool)
     if sp.causal:
         ok = j <= p[:, :, None]
@@ -428,8 +422,16 @@ def _shaped_ref(sp, q, k, v):
         d = torch.gather(sp.docs.long(), 1, p.clamp(0, Sk - 1)[..., None].expand(B, Sq, 2))
         inside = (p >= 0) & (p < Sk)
         ok = ok & inside[:, :, None] & (j >= d[..., :1]) & (j < d[..., 1:])
-    ok = ok[:, None]
-    s = s.masked_fill(~ok, float("-inf"))
+    # queries that see nothing and keys that no query sees may hold anything, forward and backward
+    sees, seen = ok.any(2)[:, :, None, None], ok.any(1)[:, :, None, None]
+    q, k, v = torch.where(sees, q, 0.0), torch.where(seen, k, 0.0), torch.where(seen, v, 0.0)
+    k, v = k.repeat_interleave(G, 2), v.repeat_interleave(G, 2)
+    s = torch.einsum("bqhd,bkhd->bhqk", q, k) * sp.scale
+    if sp.softcap:
+        s = sp.softcap * torch.tanh(s / sp.softcap)
+    if sp.slopes is not None:
+        s = s - sp.slopes[None, :, None, None] * (p[:, :, None] - j).abs()[:, None]
+    s = s.masked_fill(~ok[:, None], float("-inf"))
     m = s.amax(-1, keepdim=True)
     e = torch.exp(s - m.masked_fill(m == float("-inf"), 0.0))
     l = e.sum(-1, keepdim=True)
@@ -437,9 +439,7 @@ def _shaped_ref(sp, q, k, v):
     pr = e / l.masked_fill(l == 0, 1.0)
     if sp.p_drop > 0:
         pr = pr * dropout_keep_mask(eff_seed(sp.seed), B, H, Sq, Sk, sp.p_drop) * attn_keep_scale(sp.p_drop)
-    # keys that no query of the batch sees may hold anything
-    v = torch.where(ok[:, 0].any(1)[:, :, None, None], v, 0.0)
-    return torch.einsum("bhqk,bkhd->bqhd", pr, v), lse
+    return torch.where(sees, torch.einsum("bhqk,bkhd->bqhd", pr, v), 0.0), lse
 
 
 def _shaped_args(sp):

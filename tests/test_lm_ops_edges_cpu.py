@@ -1,0 +1,41 @@
+"""Calls of the language-model operators at their edges, on the CPU: what unseen places hold, what a plain call
+keeps, limits that are refused."""
+import math
+
+import pytest
+import torch
+
+import lm_oracle as O
+from tensorflow_k8s_amd.ops import loss as L
+from tensorflow_k8s_amd.ops import transformer as TR
+from test_lm_ops_cpu import i32, randn
+
+
+@pytest.mark.parametrize("mask", [
+    dict(kv_len=[0, 5]), dict(causal=True, q_start=[-3, 4], Sq=4), dict(causal=True, q_start=[0, 2], Sq=3),
+    dict(causal=True, doc_ids=[[4, 4, 4, 1, 1, 4, 4, -1, -1], [-1, 0, 0, 0, 0, 7, 7, 7, 7]]),
+    dict(causal=True, prefix_len=[0, 3], kv_len=[7, 2]),
+])
+@pytest.mark.parametrize("hold", [math.nan, math.inf])
+def test_attention_unseen_places_hold_anything(mask, hold):
+    """Queries that see nothing and keys that no query sees reach neither the output nor a gradient."""
+    kw = dict(mask)
+    B, H, Hk, Sk, Sq = 2, 4, 2, 9, kw.pop("Sq", 9)
+    ids = i32(kw.pop("doc_ids")) if "doc_ids" in kw else None
+    kw = {n: i32(v) if n != "causal" else v for n, v in kw.items()}
+    q, k, v = randn(B, Sq, H, 64, seed=1), randn(B, Sk, Hk, 64, seed=2), randn(B, Sk, Hk, 64, seed=3)
+    dout = randn(B, Sq, H, 64, seed=4)
+    ok, pos = O.visible(B, Sq, Sk, kw.get("causal", False), kw.get("kv_len"), kw.get("q_start"), kw.get("prefix_len"), ids)
+    blind, unseen = ~ok.any(2), ~ok.any(1)
+    assert blind.any() or unseen.any()
+    q[blind], dout[blind], k[unseen], v[unseen] = hold, hold, hold, hold
+    sp = TR.AttnSpec(B, H, Sq, Sk, (q.view(B * Sq, -1), 0), (k.view(B * Sk, -1), 0), (v.view(B * Sk, -1), 0), kv_heads=Hk,
+                     docs=TR.document_spans(ids) if ids is not None else None, softcap=6.0, **kw)
+    out, lse = TR.attention_fwd(sp)
+    g = [torch.empty_like(t[0]) for t in (sp.q, sp.k, sp.v)]
+    TR.attention_bwd(sp, out, dout.view(B * Sq, -1), lse, *((x, 0) for x in g))
+    r = O.attention(q, k, v, ok, pos, sp.scale, 6.0, None, dout)
+    O.within(out.view(r["out"].shape), r["out"], r["out_bound"], "out")
+    for n, x in zip(("dq", "dk", "dv"), g):
+        O.within(x.view(r[n].shape), r[n], r[n + "_bound"], n)
+    assert bool((lse.permute(0, 2, 1)[blind] == math.inf).all())
