@@ -61,6 +61,8 @@ struct Ty<bf16> {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
   }
   static __device__ __forceinline__ x4 tr(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS x4*)p); }
+  static constexpr bool fits = true;  // has float's exponents
+  static constexpr float p_up = 0.f;
 };
 template <>
 struct Ty<f16> {
@@ -72,6 +74,8 @@ struct Ty<f16> {
   static __device__ __forceinline__ x4 tr(const char* p) {  // 16-bit elements move as they are
     return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p));
   }
+  static constexpr bool fits = false;   // 2^-14 .. 2^16
+  static constexpr float p_up = 15.f;   // log2 of the factor that the dK/dV pass gives P <= 1: whole digits down to 2^-29
 };
 
 struct Shaped {
@@ -276,12 +280,44 @@ __device__ __forceinline__ typename Ty<T>::x8 pack8(const f32x16& a, int half) {
   return r;
 }
 
-// what pack8 leaves of a half: a - pack8(a)
+// f16 operands of the gradient products. dS = P (dP - delta) (1 - t^2) goes with 1 / keys and with the upstream gradient:
+// unscaled it left f16's range on long rows, for gradients of 1e-3 and smaller (no digits) and of 1e4 (infinite). So a
+// lane's row (dQ) or key (dK) has a power of two `up` for its dS, divided out of the f32 sums at the end: from 2^START,
+// too large for nearly any row, it falls where an element of the row would pass 2^15, to 2^12 .. 2^13 for that element, and
+// the sums so far fall with it. The largest |dS| of a lane's row or key so far is then above 2^12, and what lies 2^26
+// below it keeps all its digits. It costs an f16 backward 5 to 11% (B1 H16/4 S8192 D128 capped 1089 -> 1143 us, B2 H16
+// S2048 D64 with a bias 116 -> 130).
+constexpr float START = 0x1p60f;
+template <typename T, int D>
+__device__ __forceinline__ void fit(const f32x16& ds, float& up, f32x16 (&acc)[D / 32]) {
+  if constexpr (Ty<T>::fits) return;
+  float mx = fabsf(ds[0]);
+#pragma unroll
+  for (int e = 1; e < 16; ++e) mx = fmaxf(mx, fabsf(ds[e]));
+  mx = pair_max(mx) * up;
+  if (!__any(mx > 0x1p15f)) return;
+  const float f = ldexpf(1.f, mx > 0x1p15f ? min(13 - __builtin_amdgcn_frexp_expf(mx), 0) : 0);  // (inf: stays)
+  up *= f;
+#pragma unroll
+  for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[db][e] *= f;
+}
+// 1 / up, exactly
+__device__ __forceinline__ float down(float up) { return __uint_as_float((254u << 23) - __float_as_uint(up)); }
 template <typename T>
-__device__ __forceinline__ typename Ty<T>::x8 pack8_rest(const f32x16& a, int half, typename Ty<T>::x8 hi) {
+__device__ __forceinline__ typename Ty<T>::x8 pack8(const f32x16& a, int half, float up) {
   typename Ty<T>::x8 r;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = (T)(a[8 * half + e] - (float)hi[e]);
+  for (int e = 0; e < 8; ++e) r[e] = (T)(Ty<T>::fits ? a[8 * half + e] : a[8 * half + e] * up);
+  return r;
+}
+// what pack8 leaves of a half: a up - pack8(a, up)
+template <typename T>
+__device__ __forceinline__ typename Ty<T>::x8 pack8_rest(const f32x16& a, int half, float up, typename Ty<T>::x8 hi) {
+  typename Ty<T>::x8 r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)((Ty<T>::fits ? a[8 * half + e] : a[8 * half + e] * up) - (float)hi[e]);
   return r;
 }
 

@@ -5,7 +5,7 @@
 
 namespace {
 // ------------------------------------------------------------------------------- dQ pass
-// same rows and tiles as the forward; also writes lse in log2 units (shifted, Score) and -delta.
+// same rows and tiles as the forward; also writes lse in log2 units (shifted, Score; f16: less p_up) and -delta.
 // Precision: delta = sum P dP is taken as dO.O here, off by O's rounding. Beside the roundings of dS and of the
 // gradients this weighs as much as they do where a row's softmax rests on few keys, 1 / n_eff of it else (974 keys
 // under a slope of 1/2 gave 1.7 times the error of a float32 backward, 372 without one 1.48). So where a row of the
@@ -13,8 +13,10 @@ namespace {
 // error, corrects the delta of the dK/dV pass, and dQ, where it stays, takes dS into its product as two 16-bit
 // terms. (Everywhere: B1 H16/4 S8192 D128 dQ 417 -> 580 us, B4 H16 S2048 D64 documents 35 -> 41.)
 constexpr int FEW = 128;
+// (168 registers are not enough for dropout's hashes beside f16's running scale)
+constexpr int dq_min_waves(int D, bool drop, bool fits) { return D == 64 && (fits || !drop) ? 3 : 2; }
 template <typename T, int D, int NW, typename O>
-__global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Shaped p) {
+__global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) void shaped_dq_kernel(Shaped p) {
   constexpr bool DOCS = O::docs;
   constexpr int KT = key_tile(D), TB = KT * D * 2;
   typedef DeadRows<D, NW, KT> Dead;
@@ -95,6 +97,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   const int qg = (q >> 2) * p.Sk;
   const bool two = __any(sees && (sp.hi - sp.lo <= FEW || (O::bias && slope * FEW >= 2.f * LOG2E)));  // e^-2 at FEW
   float rest = 0.f;  // this lane's half of sum P (dP - delta)
+  float up = START;
   f32x16 acc[D / 32], ndl;  // -delta in every slot: dP - delta is the product's start
 #pragma unroll
   for (int e = 0; e < 16; ++e) ndl[e] = -dlt;
@@ -146,13 +149,14 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= dp[e];
       }
+      fit<T, D>(s, up, acc);
 #pragma unroll
       for (int kc = 0; kc < 2; ++kc) {
-        const typename Ty<T>::x8 hi = pack8<T>(s, kc);
+        const typename Ty<T>::x8 hi = pack8<T>(s, kc, up);
 #pragma unroll
         for (int db = 0; db < D / 32; ++db) acc[db] = Ty<T>::mfma(frag_tr<T, D>(smem, KA, fo, 2 * kb + kc, db), hi, acc[db]);
         if (two) {
-          const typename Ty<T>::x8 lo = pack8_rest<T>(s, kc, hi);
+          const typename Ty<T>::x8 lo = pack8_rest<T>(s, kc, up, hi);
 #pragma unroll
           for (int db = 0; db < D / 32; ++db) acc[db] = Ty<T>::mfma(frag_tr<T, D>(smem, KA, fo, 2 * kb + kc, db), lo, acc[db]);
         }
@@ -166,11 +170,11 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 3 : 2) void shaped_dq_kernel(Sha
   }
   rest = xor_sum<32>(rest);
   if (valid && h == 0) {  // for the dK/dV pass
-    p.delta[srow_i] = lse2;
+    p.delta[srow_i] = lse2 - Ty<T>::p_up;
     p.delta[(long long)p.B * p.H * p.Sq + srow_i] = -(dlt + rest);
   }
   if (valid) {
-    const float f = O::cap ? 4.f * p.scale : p.scale;
+    const float f = (O::cap ? 4.f * p.scale : p.scale) * (Ty<T>::fits ? 1.f : down(up));
     T* dQ = (T*)p.dq + b * p.dq_bs + q * p.dq_rs + head * D + 4 * h;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
@@ -294,6 +298,7 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[db][e] = dv[db][e] = 0.f;
+  float up = START * (Ty<T>::fits ? 1.f : 0x1p-15f);  // (f16: P, and with it dS, is 2^15 times itself here)
   int g = i0 / max(nt, 1), t = i0 % max(nt, 1);
   if (i0 < i1) landed(0, org + t * KT);
   auto step = [&](auto slot_, int i) {
@@ -377,10 +382,11 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
             for (int e = 0; e < 4; ++e) s[4 * u + e] = (kp & (1u << e)) ? s[4 * u + e] : 0.f;
           }
         }
+        fit<T, D>(dp, up, dk);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int kc = 0; kc < 2; ++kc) {
-          const typename Ty<T>::x8 pf = pack8<T>(s, kc), sf = pack8<T>(dp, kc);
+          const typename Ty<T>::x8 pf = pack8<T>(s, kc), sf = pack8<T>(dp, kc, up);
 #pragma unroll
           for (int db = 0; db < D / 32; ++db) {
             dv[db] = Ty<T>::mfma(frag_tr<T, D>(smem, OA, fo, 2 * qb_ + kc, db), pf, dv[db]);
@@ -398,6 +404,16 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   for (int i = i0; i < i1; i += 2) {
     step(iconst<0>{}, i);
     if (i + 1 < i1) step(iconst<1>{}, i + 1);
+  }
+  if constexpr (!Ty<T>::fits) {
+    const float fk = down(up) * 0x1p-15f;
+#pragma unroll
+    for (int db = 0; db < D / 32; ++db)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        dk[db][e] *= fk;
+        dv[db][e] *= 0x1p-15f;
+      }
   }
   if (splits > 1) {
     if (key >= p.Sk) return;

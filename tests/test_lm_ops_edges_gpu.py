@@ -50,3 +50,38 @@ def test_attention_divided_cache(name):
     c.q[dead_q] = math.nan  # rows and keys that no pair uses hold anything
     c.k[dead_k], c.v[dead_k] = math.nan, math.inf
     c.check(grads=False)  # (0 and lse +inf where a row sees nothing)
+
+
+# ------------------------------------------------------------------------------------- half precision gradients
+
+@pytest.mark.parametrize("scale", [1e4, 1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("kind", ["long", "long_wide", "long_documents", "first_keys"])
+def test_attention_f16_gradients_at_any_scale(kind, cap, scale):
+    """f16 gradients of small and large upstream gradients: P (dP - delta) is far below the smallest f16 number, or above
+    the largest, where the gradients themselves are not. The relative 2-norm of the error is at most that of two
+    roundings, sqrt(2) times that of the exact gradient rounded once (and 6% for the rest)."""
+    c = {"long": lambda: Case(B=1, H=2, Hk=1, Sq=2100, causal=True, cap=cap, dtype=HF),
+         "long_wide": lambda: Case(B=1, H=1, D=128, Sq=300, Sk=2300, cap=cap, dtype=HF, fused=False),
+         "long_documents": lambda: Case(B=1, H=2, Sq=2000, cap=cap, dtype=HF, slopes=0.01, doc_ids=docs(1, 2000, [1500, 400])),
+         "first_keys": lambda: Case(B=2, H=2, D=128, Sq=90, causal=True, cap=cap, dtype=HF)}[kind]()
+    c.dout = (c.dout.float() * scale).to(HF)
+    r, sp = c.oracle(), c.spec()
+    out, lse = TR.attention_fwd(sp)
+    g = [torch.empty(c.B * S, n * c.D, dtype=HF, device=DEV) for S, n in ((c.Sq, c.H), (c.Sk, c.Hk), (c.Sk, c.Hk))]
+    TR.attention_bwd(sp, out, c.dout.reshape(c.B * c.Sq, -1).to(DEV), lse, *((x, 0) for x in g))
+    for n, x in zip(("dq", "dk", "dv"), g):
+        w = r[n]
+        once = (w.to(HF).double() - w).norm()
+        assert torch.isfinite(once)
+        assert (x.view(w.shape).double().cpu() - w).norm() <= 1.5 * once, n
+
+
+@pytest.mark.parametrize("kw", [
+    dict(B=2, H=2, Sq=130, causal=True, cap=7.0, p_drop=0.2, doc_ids=docs(2, 130, [100, 9])),
+    dict(B=1, H=4, Hk=2, D=128, Sq=35, Sk=70, p_drop=0.5, fused=False, slopes=True),
+    dict(B=1, H=2, Hk=1, D=128, Sq=300, causal=True, p_drop=0.1),
+    dict(B=2, H=4, Hk=2, Sq=3, Sk=90, causal=True, q_start=[87, 30], p_drop=0.3, fused=False),
+])
+def test_attention_f16_dropout(kw):
+    Case(dtype=HF, **kw).check()
