@@ -101,8 +101,9 @@ void check_shape(const std::vector<int64_t>& s, double scale, double cap, double
   // query rows padded to whole tiles (of up to 256); block counts and row indices are 32-bit
   TORCH_CHECK(s[0] * s[1] <= 0x7fffffff && (s[3] + 256) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x7ffffff, "attention shape too large");
   TORCH_CHECK(((s[3] + 256) / 32 * (s[1] / s[2]) + s[4] / 64 + 2) * s[0] * s[2] <= 0x7fffffff, "attention grid too large");
-  TORCH_CHECK(scale > 0.0 && std::isfinite(scale), "scale must be positive, got ", scale);
-  TORCH_CHECK(cap >= 0.0 && std::isfinite(cap), "softcap must be >= 0, got ", cap);
+  // (within float32's whole-digit range)
+  TORCH_CHECK(scale >= 1.2e-38 && scale <= 2e38, "scale must be positive, got ", scale);
+  TORCH_CHECK(cap == 0.0 || (cap >= 1.2e-38 && cap <= 2e38), "softcap must be >= 0, got ", cap);
   TORCH_CHECK(p_drop >= 0.0 && p_drop < 1.0, "p_drop");
 }
 struct Masks {

@@ -96,24 +96,35 @@ struct Shaped {
   const unsigned long long* seed_key;
 };
 
+// Caps up to here take the shifted form of a score (Score), larger ones the wide form. The shift puts the float32 step of
+// cap on every score: f16, S 600, relative error of O (0.00020: rounded once) and absolute one of lse are 0.000256 and 1e-5 at
+// a cap of 128, 0.000255 and 4e-5 at 512, 0.000258 and 6e-5 at 1024, 0.00049 and 7e-4 at 1e4, 0.0037 and 8e-3 at 1e5; the
+// wide form's 0.000254 and 1e-6 at any cap, for up to half more time (B1 H16/4 S8192 D128 bf16:
+// forward 351 -> 540 us, backward 1021 -> 1323).
+constexpr float CAP_SHIFT = 512.f;
+__host__ __device__ __forceinline__ bool shifted(const Shaped& p) { return p.cap > 0.f && p.cap <= CAP_SHIFT; }
+
 // the score rules of a call, compiled in: as runtime branches their joins cost the dK/dV pass 40 registers
-template <bool DOCS, bool CAP, bool BIAS, bool DROP>
+enum Cap { NONE, SHIFTED, WIDE };
+template <bool DOCS, Cap CAP, bool BIAS, bool DROP>
 struct Rules {
-  static constexpr bool docs = DOCS, cap = CAP, bias = BIAS, drop = DROP;
+  static constexpr bool docs = DOCS, cap = CAP == SHIFTED, wide = CAP == WIDE, bias = BIAS, drop = DROP;
 };
 template <typename F>
 void with_rules(const Shaped& p, F f) {
   auto dr = [&](auto docs, auto cap, auto bias) {
-    if (p.p_drop > 0.f) f(Rules<docs.value, cap.value, bias.value, true>{});
-    else f(Rules<docs.value, cap.value, bias.value, false>{});
+    constexpr Cap C = (Cap)decltype(cap)::value;
+    if (p.p_drop > 0.f) f(Rules<docs.value, C, bias.value, true>{});
+    else f(Rules<docs.value, C, bias.value, false>{});
   };
   auto bi = [&](auto docs, auto cap) {
     if (p.slopes) dr(docs, cap, bconst<true>{});
     else dr(docs, cap, bconst<false>{});
   };
   auto ca = [&](auto docs) {
-    if (p.cap > 0.f) bi(docs, bconst<true>{});
-    else bi(docs, bconst<false>{});
+    if (p.cap > CAP_SHIFT) dr(docs, iconst<WIDE>{}, bconst<true>{});  // slopes: perhaps 0
+    else if (p.cap > 0.f) bi(docs, iconst<SHIFTED>{});
+    else bi(docs, iconst<NONE>{});
   };
   if (p.docs) ca(bconst<true>{});
   else ca(bconst<false>{});
@@ -373,18 +384,36 @@ struct Dma {
 // plain: x = s scale log2e. Capped: cap tanh(u) = cap - 2 cap r with r = 1 / (1 + e^2u), u = s scale / cap; the
 // constant cap shifts a whole row, so x = -2 cap log2e r, and d tanh = 1 - tanh^2 = 4 (r - r^2). Distances add
 // -slope log2e |p - j|. (Row statistics between the passes are in these shifted units.)
+// Wide caps: x = cap log2e t without a shift, t = tanh(u) to a few of its own steps: the Taylor series up to u^9 where
+// |u| < 1/4 (the next term is below 2^-26 of it), else 1 - 2 r of |u| with u's sign.
 template <typename O>
 struct Score {
   float c2, c2l, mult, base;  // 2 log2e scale / cap, -2 cap log2e, scale log2e, the shift
+  float cu, cl;               // wide: scale / cap, cap log2e
   __device__ __forceinline__ Score(const Shaped& p) {
     mult = p.scale * LOG2E;
-    c2 = O::cap ? 2.f * mult / p.cap : 0.f;
+    c2 = O::cap ? fminf(2.f * mult / p.cap, 3.4e38f) : 0.f;
     base = O::cap ? p.cap * LOG2E : 0.f;
     c2l = -2.f * base;
+    const float wide = fminf(p.cap, 1e30f);  // (leaves any score below 1e26 alone)
+    cu = O::wide ? p.scale / wide : 0.f;
+    cl = O::wide ? wide * LOG2E : 0.f;
   }
+  __device__ __forceinline__ float t(float s) const {
+    const float u = s * cu, w = u * u;
+    const float series = fmaf(w, fmaf(w, fmaf(w, fmaf(w, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+    const float far = fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + ex2(fabsf(u) * (2.f * LOG2E))), 1.f);
+    return fabsf(u) < 0.25f ? u * series : copysignf(far, u);
+  }
+  // a score without its distance
+  __device__ __forceinline__ float x(float s) const { return O::wide ? cl * t(s) : O::cap ? c2l * r(s) : s * mult; }
   // native exp2 and reciprocal: saturates through e = inf (r = 0) and e = 0 (r = 1)
   __device__ __forceinline__ float r(float s) const { return __builtin_amdgcn_rcpf(1.f + ex2(s * c2)); }
 };
+template <typename O>
+__device__ __forceinline__ float slope_of(const Shaped& p, int head) {
+  return O::bias && (!O::wide || p.slopes) ? p.slopes[head] * LOG2E : 0.f;
+}
 // slot r of a 32-row block: row (r & 3) + 8 (r >> 2) (+ 4 h)
 __device__ __forceinline__ constexpr int srow(int r) { return (r & 3) + 8 * (r >> 2); }
 

@@ -88,7 +88,7 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
   const long long srow_i = ((long long)b * p.H + head) * p.Sq + qc;
   const Score<O> sc(p);
   const float lse2 = sees ? fmaf(p.lse[srow_i], LOG2E, -sc.base) : INFINITY;
-  const float slope = O::bias ? p.slopes[head] * LOG2E : 0.f;
+  const float slope = slope_of<O>(p, head);
   const int pos = q + mk.shift;
   const int thr = drop_thr(p.p_drop);
   constexpr bool drop = O::drop;
@@ -129,14 +129,15 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
           for (int u = 0; u < 4; ++u) dp[e + u] = fmaf((kp & (1u << u)) ? dp[e + u] + dlt : 0.f, keep, -dlt);
         }
       }
-      // P (dP - delta) in s; capped: d tanh / 4 in dp
+      // P (dP - delta) in s; capped: d tanh / 4 (wide: d tanh) in dp
       const float d0 = O::bias ? (float)(pos - k0 - 4 * h) : 0.f;
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const float r_ = O::cap ? sc.r(s[e]) : 0.f;
-        const float x = O::cap ? fmaf(r_, sc.c2l, -lse2) : fmaf(s[e], sc.mult, -lse2);
+        const float r_ = O::wide ? sc.t(s[e]) : O::cap ? sc.r(s[e]) : 0.f;
+        const float x = O::wide ? fmaf(r_, sc.cl, -lse2) : O::cap ? fmaf(r_, sc.c2l, -lse2) : fmaf(s[e], sc.mult, -lse2);
         s[e] = ex2(O::bias ? fmaf(-slope, fabsf(d0 - (float)srow(e)), x) : x) * dp[e];
         if (O::cap) dp[e] = fmaf(-r_, r_, r_);
+        if (O::wide) dp[e] = fmaf(-r_, r_, 1.f);
       }
       if (!(k0 >= re.ilo && k0 + 32 <= re.ihi)) mask_slots(s, (unsigned)(k0 + 4 * h - sp.lo), (unsigned)(sp.hi - sp.lo), 0.f);
       if (two) {
@@ -145,7 +146,7 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
         for (int e = 4; e < 16; e += 4) { a += s[e] + s[e + 1]; b_ += s[e + 2] + s[e + 3]; }
         rest += a + b_;
       }
-      if (O::cap) {
+      if (O::cap || O::wide) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] *= dp[e];
       }
@@ -193,7 +194,7 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
 // hashes 256 registers are not enough at D = 128
 constexpr int dkv_waves(int D, bool drop) { return D == 128 && !drop ? 8 : 4; }
 constexpr int dkv_min_waves(int D, bool drop) { return D == 64 ? (drop ? 2 : 3) : (drop ? 1 : 2); }
-__device__ __forceinline__ float dk_scale(const Shaped& p) { return p.cap > 0.f ? 4.f * p.scale : p.scale; }  // d tanh's 4
+__device__ __forceinline__ float dk_scale(const Shaped& p) { return shifted(p) ? 4.f * p.scale : p.scale; }  // d tanh's 4
 // NW waves of 32 keys; streams the query tiles of all G heads of the group (or, with `splits`, an even share of
 // them: then f32 sums go to `part` and shaped_dkv_join_kernel adds them in order). The block's K rows stay in
 // LDS instead of registers: at D = 128 the two accumulators take 128 registers, and K's 32 more made the
@@ -305,7 +306,7 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
     constexpr int slot = decltype(slot_)::value, QA = slot * 2 * TB, OA = QA + TB;
     const int q0 = org + t * KT, head = hk * p.G + g;
     if (i + 1 < i1) issue(slot ^ 1);
-    const float slope = O::bias ? p.slopes[head] * LOG2E : 0.f;
+    const float slope = slope_of<O>(p, head);
     const uint32_t hs = drop ? head_seed(p, b * p.H + head) : 0u;
     const bool full = all_seen && q0 >= re.ilo && q0 + KT <= re.ihi;
     if (q0 < re.uhi && q0 + KT > re.ulo) {  // wave-uniform
@@ -348,6 +349,11 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
               const float r_ = sc.r(s[e]);
               x = sc.c2l * r_;
               dp[e] *= fmaf(-r_, r_, r_);
+            }
+            if (O::wide) {
+              const float t_ = sc.t(s[e]);
+              x = sc.cl * t_;
+              dp[e] *= fmaf(-t_, t_, 1.f);
             }
             s[e] = ex2(fmaf(-slope, fabsf(d0 + (float)srow(e)), x - Lr[srow(e)]));
             dp[e] *= s[e];

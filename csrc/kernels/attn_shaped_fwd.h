@@ -67,7 +67,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) qf[kk] = frag_mem<T>(Qr, kk, sees);
   const Score<O> sc(p);
-  const float slope = O::bias ? p.slopes[head] * LOG2E : 0.f;
+  const float slope = slope_of<O>(p, head);
   const int pos = q + mk.shift;
   const int thr = drop_thr(p.p_drop);
   constexpr bool drop = O::drop;
@@ -97,7 +97,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
         const float d0 = (float)(pos - k0 - 4 * h);
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          s[e] = fmaf(-slope, fabsf(d0 - (float)srow(e)), O::cap ? sc.c2l * sc.r(s[e]) : s[e] * sc.mult);
+          s[e] = fmaf(-slope, fabsf(d0 - (float)srow(e)), sc.x(s[e]));
       }
       if (part) mask_slots(s, (unsigned)(k0 + 4 * h - sp.lo), (unsigned)(sp.hi - sp.lo), -INFINITY);
       // the row maximum of the raw products (a score grows with its product; distances: of the scores)
@@ -241,9 +241,9 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
 #pragma unroll
   for (int kk = 0; kk < D / 16; ++kk) qf[kk] = frag_mem<T>(Qr, kk, sees);
   const Score<O> sc(p);
-  const float slope = O::bias ? p.slopes[head] * LOG2E : 0.f;
+  const float slope = slope_of<O>(p, head);
   const int pos = q + mk.shift;
-  const float fs = O::cap ? 1.f : sc.mult, fx = O::bias ? 1.f : fs;  // factors left to the bias, to the exponent
+  const float fs = O::cap || O::wide ? 1.f : sc.mult, fx = O::bias ? 1.f : fs;  // factors left to the bias, to the exponent
   float m = -INFINITY, lsum = 0.f;
   f32x16 o[D / 32];
 #pragma unroll
@@ -271,11 +271,11 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
     __builtin_amdgcn_wave_barrier();
     if (t + FW < t1) load(t + FW);
     // (maximum of the finished scores: few rows are bound by memory, and this path is the shortest code)
-    if (O::cap) {
+    if (O::cap || O::wide) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] = sc.c2l * sc.r(s[kb][e]);
+        for (int e = 0; e < 16; ++e) s[kb][e] = sc.x(s[kb][e]);
     }
     if (O::bias) {
       const float d0 = (float)(pos - k0 - 4 * h);
@@ -411,7 +411,7 @@ __global__ __launch_bounds__(64) void shaped_few_join_kernel(Shaped p, int split
   T* Or = (T*)p.out + b * p.o_bs + q * p.o_rs + head * D;
 #pragma unroll
   for (int u = 0; u < D / 64; ++u) Or[u * 64 + l] = (T)(o[u] * inv);
-  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + (p.cap > 0.f ? p.cap * LOG2E : 0.f) + __log2f(L)) * LN2 : INFINITY;
+  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + (shifted(p) ? p.cap * LOG2E : 0.f) + __log2f(L)) * LN2 : INFINITY;
 }
 
 // few rows and no dropout: the split form; shares of a cache so that there are about 4 blocks for each of

@@ -364,10 +364,10 @@ class AttnSpec:
             raise ValueError(f"attention: {self.H} heads do not share {self.kv_heads} key heads evenly")
         if min(self.B, self.Sq, self.Sk) < 1:
             raise ValueError(f"attention: empty shape B={self.B} Sq={self.Sq} Sk={self.Sk}")
-        if not (math.isfinite(self.softcap) and self.softcap >= 0.0):
-            raise ValueError(f"attention: softcap must be >= 0, got {self.softcap}")
-        if not (math.isfinite(self.scale) and self.scale > 0.0):
-            raise ValueError(f"attention: scale must be positive, got {self.scale}")
+        if not (self.softcap == 0.0 or 1.2e-38 <= self.softcap <= 2e38):  # float32 holds it with all digits
+            raise ValueError(f"attention: softcap must be >= 0 (0 or 1.2e-38 to 2e38), got {self.softcap}")
+        if not 1.2e-38 <= self.scale <= 2e38:
+            raise ValueError(f"attention: scale must be positive (1.2e-38 to 2e38), got {self.scale}")
         if self.prefix_len is not None and not self.causal:
             raise ValueError("attention: prefix_len needs causal=True")
         B = (self.B,)

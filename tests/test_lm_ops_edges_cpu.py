@@ -39,3 +39,12 @@ def test_attention_unseen_places_hold_anything(mask, hold):
     for n, x in zip(("dq", "dk", "dv"), g):
         O.within(x.view(r[n].shape), r[n], r[n + "_bound"], n)
     assert bool((lse.permute(0, 2, 1)[blind] == math.inf).all())
+
+
+@pytest.mark.parametrize("kw", [dict(softcap=1e-46), dict(softcap=1e39), dict(softcap=1.0, scale=1e-46), dict(softcap=1.0, scale=1e39),
+                                dict(softcap=math.nan), dict(softcap=1.0, scale=math.nan)])
+def test_attention_refuses_what_float32_does_not_hold(kw):
+    """(1e-46 is 0 and 1e39 infinite in float32)"""
+    q = randn(16, 128)
+    with pytest.raises(ValueError):
+        TR.AttnSpec(2, 2, 8, 8, (q, 0), (q, 0), (q, 0), **kw)

@@ -85,3 +85,24 @@ def test_attention_f16_gradients_at_any_scale(kind, cap, scale):
 ])
 def test_attention_f16_dropout(kw):
     Case(dtype=HF, **kw).check()
+
+
+# ------------------------------------------------------------------------------------- any score cap
+
+@pytest.mark.parametrize("cap", [1.2e-38, 1e-30, 1e-3, 128.0, 512.0, 513.0, 1e4, 1e6, 1e8, 1e30, 2e38])
+@pytest.mark.parametrize("kw", [
+    dict(B=1, H=2, Hk=1, Sq=150, causal=True),
+    dict(B=1, H=2, Hk=1, D=128, Sq=140, causal=True, dtype=HF, slopes=True, doc_ids=docs(1, 140, [60, 29], pad=7)),
+    dict(B=2, H=2, Sq=90, Sk=120, kv_len=[120, 40], fused=False, p_drop=0.2),
+    dict(B=1, H=1, Sq=100, causal=True, scale=8.0),  # scores of some hundreds: where a cap of 512 still acts
+], ids=["causal", "f16_docs_bias", "dropout", "large_scores"])
+def test_attention_any_cap(kw, cap):
+    """Small and large caps: scores, lse and gradients as exact as without a cap (a large cap leaves the scores alone)."""
+    Case(cap=cap, **kw).check()
+
+
+@pytest.mark.parametrize("cap", [1e-30, 512.0, 513.0, 1e6, 1e30])
+@pytest.mark.parametrize("Sk", [300, 1500])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_attention_any_cap_few_rows(dtype, Sk, cap):
+    Case(B=2, H=4, Hk=2, D=128, Sq=2, Sk=Sk, causal=True, kv_len=[Sk, 9], q_start=[Sk - 2, 7], cap=cap, dtype=dtype, fused=False).check(grads=False)
