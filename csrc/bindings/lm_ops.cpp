@@ -69,7 +69,7 @@ void check_cols(const torch::Tensor& t, const torch::Tensor& ref, long long off,
   TORCH_CHECK(t.dim() >= 2 && (t.size(-1) == 1 || t.stride(-1) == 1), n, " needs unit stride along its last dim");
   TORCH_CHECK(off >= 0 && off + W <= t.size(-1), n, ": columns ", off, "..", off + W, " outside a width of ", t.size(-1));
   TORCH_CHECK(rs % 8 == 0 && bs % 8 == 0 && off % 8 == 0, n, ": strides/offset must be multiples of 8 elements");
-  TORCH_CHECK((rs >= W || S == 1) && rs < (1 << 23), n, ": token stride ", rs, " not in ", W, "..2^23");
+  TORCH_CHECK(rs >= W && rs < (1 << 23), n, ": token stride ", rs, " not in ", W, "..2^23");
   const long long have = (long long)(t.storage().nbytes() / t.element_size()) - t.storage_offset();
   TORCH_CHECK(bs >= 0 && off + (B - 1) * bs + (S - 1) * rs + W <= have, n, " too small for its shape");
   TORCH_CHECK((reinterpret_cast<uintptr_t>(t.data_ptr()) + 2 * off) % 16 == 0, n, " must be 16-byte aligned");
@@ -122,11 +122,15 @@ Masks masks(const Opt& kv_len, const Opt& q_start, const Opt& prefix, const Opt&
                opt_ptr<const int>(docs), opt_ptr<const float>(slopes)};
 }
 
-// [batch, token] strides of a 2-D [B * S, width] or 3-D [B, S', width] buffer
-void buf_strides(const torch::Tensor& t, long long S, long long* st, const char* n) {
+// [batch, token] strides of a 2-D [B * S, width] or 3-D [B, S', width] buffer that holds W columns. The stride of a single
+// token or batch says nothing (an expanded view's is 0, and a tile is read through a descriptor of rows times stride
+// bytes): as in a tight buffer.
+void buf_strides(const torch::Tensor& t, long long B, long long S, long long W, long long* st, const char* n) {
   TORCH_CHECK(t.dim() == 2 || t.dim() == 3, n, " must be [B*S, width] or [B, S', width]");
   st[1] = t.stride(-2);
   st[0] = t.dim() == 3 ? t.stride(0) : S * st[1];
+  if (S == 1) st[1] = W;
+  if (B == 1) st[0] = S * st[1];
 }
 struct Call {
   int f16;
@@ -140,9 +144,9 @@ Call check_call(const torch::Tensor& q, int64_t qo, const torch::Tensor& k, int6
   check_shape(shape, scale, cap, p_drop);
   for (int i = 0; i < 6; ++i) c.sh[i] = shape[i];
   const long long B = shape[0], H = shape[1], Hk = shape[2], Sq = shape[3], Sk = shape[4], D = shape[5];
-  buf_strides(q, Sq, c.st, "q");
-  buf_strides(k, Sk, c.st + 2, "k");
-  buf_strides(v, Sk, c.st + 4, "v");
+  buf_strides(q, B, Sq, H * D, c.st, "q");
+  buf_strides(k, B, Sk, Hk * D, c.st + 2, "k");
+  buf_strides(v, B, Sk, Hk * D, c.st + 4, "v");
   c.st[6] = Sq * H * D;
   c.st[7] = H * D;
   check_cols(q, q, qo, c.st[0], c.st[1], B, Sq, H * D, false, "q");
@@ -178,9 +182,9 @@ void shaped_bwd(torch::Tensor q, int64_t qo, torch::Tensor k, int64_t ko, torch:
   const c10::DeviceGuard guard(q.device());
   const long long B = shape[0], H = shape[1], Hk = shape[2], Sq = shape[3], Sk = shape[4], D = shape[5];
   long long gs[6];
-  buf_strides(dq, Sq, gs, "dq");
-  buf_strides(dk, Sk, gs + 2, "dk");
-  buf_strides(dv, Sk, gs + 4, "dv");
+  buf_strides(dq, B, Sq, H * D, gs, "dq");
+  buf_strides(dk, B, Sk, Hk * D, gs + 2, "dk");
+  buf_strides(dv, B, Sk, Hk * D, gs + 4, "dv");
   TORCH_CHECK(out.is_contiguous() && dout.is_contiguous(), "out and dout must be contiguous [B*Sq, H*D]");
   check_cols(out, q, 0, c.st[6], c.st[7], B, Sq, H * D, false, "out");
   check_cols(dout, q, 0, c.st[6], c.st[7], B, Sq, H * D, false, "dout");

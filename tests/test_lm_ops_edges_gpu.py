@@ -106,3 +106,27 @@ def test_attention_any_cap(kw, cap):
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_attention_any_cap_few_rows(dtype, Sk, cap):
     Case(B=2, H=4, Hk=2, D=128, Sq=2, Sk=Sk, causal=True, kv_len=[Sk, 9], q_start=[Sk - 2, 7], cap=cap, dtype=dtype, fused=False).check(grads=False)
+
+
+# ------------------------------------------------------------------------------------- strides of lone tokens
+
+def test_attention_lone_tokens_of_any_stride():
+    """Sequences of one token: the stride of that dim says nothing, whatever it is (0 in an expanded view)."""
+    c = Case(B=3, H=4, Hk=2, Sq=1, Sk=1, cap=3.0, fused=False)
+    sp = c.spec()
+    k, v = sp.k[0][:1], sp.v[0][:1]
+    for shared in (lambda t: t.expand(3, 128), lambda t: t.unsqueeze(0).expand(3, 1, 128),
+                   lambda t: torch.as_strided(t, (3, 1, 128), (0, 8, 1))):
+        a = TR.AttnSpec(3, 4, 1, 1, sp.q, (shared(k), 0), (shared(v), 0), kv_heads=2, softcap=3.0)
+        b = TR.AttnSpec(3, 4, 1, 1, sp.q, (k.repeat(3, 1), 0), (v.repeat(3, 1), 0), kv_heads=2, softcap=3.0)
+        res = []
+        for s in (a, b):
+            out, lse = TR.attention_fwd(s)
+            g = [torch.empty(3, n, dtype=BF, device=DEV) for n in (256, 128, 128)]
+            TR.attention_bwd(s, out, c.dout.reshape(3, -1).to(DEV), lse, *((x, 0) for x in g))
+            res.append([out, lse] + g)
+        assert bool(res[1][0].any()) and all(torch.equal(x, y) for x, y in zip(*res))
+    one = torch.as_strided(sp.k[0], (1, 1, 128), (128, 8, 1)), torch.as_strided(sp.v[0], (1, 1, 128), (128, 0, 1))
+    a = TR.AttnSpec(1, 4, 3, 1, (sp.q[0][:3], 0), (one[0], 0), (one[1], 0), kv_heads=2, softcap=3.0)
+    b = TR.AttnSpec(1, 4, 3, 1, (sp.q[0][:3], 0), (k, 0), (v, 0), kv_heads=2, softcap=3.0)
+    assert all(torch.equal(x, y) for x, y in zip(TR.attention_fwd(a), TR.attention_fwd(b)))
