@@ -9,7 +9,7 @@ namespace {
 // Precision: delta = sum P dP is taken as dO.O here, off by O's rounding. Beside the roundings of dS and of the
 // gradients this weighs as much as they do where a row's softmax rests on few keys, 1 / n_eff of it else (974 keys
 // under a slope of 1/2 gave 1.7 times the error of a float32 backward, 372 without one 1.48). So where a row of the
-// wave sees at most FEW keys, or its slope leaves it about as many, sum P (dP - delta) over the row, which is that
+// wave sees at most FEW keys, or its slope of either sign leaves it about as many, sum P (dP - delta) over the row, which is that
 // error, corrects the delta of the dK/dV pass, and dQ, where it stays, takes dS into its product as two 16-bit
 // terms. (Everywhere: B1 H16/4 S8192 D128 dQ 417 -> 580 us, B4 H16 S2048 D64 documents 35 -> 41.)
 constexpr int FEW = 128;
@@ -95,7 +95,7 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
   const float keep = drop ? 256.f / (float)(256 - thr) : 1.f;
   const uint32_t hs = drop ? head_seed(p, b * p.H + head) : 0u;
   const int qg = (q >> 2) * p.Sk;
-  const bool two = __any(sees && (sp.hi - sp.lo <= FEW || (O::bias && slope * FEW >= 2.f * LOG2E)));  // e^-2 at FEW
+  const bool two = __any(sees && (sp.hi - sp.lo <= FEW || (O::bias && fabsf(slope) * FEW >= 2.f * LOG2E)));  // e^-2 at FEW
   float rest = 0.f;  // this lane's half of sum P (dP - delta)
   float up = START;
   f32x16 acc[D / 32], ndl;  // -delta in every slot: dP - delta is the product's start

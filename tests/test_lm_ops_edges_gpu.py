@@ -130,3 +130,31 @@ def test_attention_lone_tokens_of_any_stride():
     a = TR.AttnSpec(1, 4, 3, 1, (sp.q[0][:3], 0), (one[0], 0), (one[1], 0), kv_heads=2, softcap=3.0)
     b = TR.AttnSpec(1, 4, 3, 1, (sp.q[0][:3], 0), (k, 0), (v, 0), kv_heads=2, softcap=3.0)
     assert all(torch.equal(x, y) for x, y in zip(TR.attention_fwd(a), TR.attention_fwd(b)))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("slope", [1.0, -1.0])
+def test_attention_gradients_under_steep_slopes(slope, dtype):
+    """Rows that rest on few keys, near ones or (negative slopes) the farthest: each gradient keeps to two roundings.
+    dK and dV: sqrt(2) times the error of the exact gradient rounded once (and 6%). dQ takes delta = dO.out from the
+    rounded out that the backward is given, so row i is off by scale e_i sum_j P_ij K_j with e_i = dO_i.(out_i - O_i),
+    beside its own rounding: both are known here, their squares add. (With a negative slope all rows rest on the same
+    three keys, so the ratio of the two is one draw, not a mean: 1.5 times one rounding does not bound it.)"""
+    c = Case(B=1, H=1, D=128, Sq=400, causal=True, dtype=dtype, slopes=slope)
+    r, sp = c.oracle(), c.spec()
+    out, lse = TR.attention_fwd(sp)
+    g = [torch.empty(400, 128, dtype=dtype, device=DEV) for _ in range(3)]
+    TR.attention_bwd(sp, out, c.dout.reshape(400, -1).to(DEV), lse, *((x, 0) for x in g))
+    Q, K = c.q[0, :, 0].double(), c.k[0, :, 0].double()
+    scale = 1 / math.sqrt(128)
+    z = (Q @ K.T) * scale - c.slopes[0].double() * (torch.arange(400)[:, None] - torch.arange(400)).abs()
+    p = torch.softmax(z.masked_fill(~c.ok[0], -math.inf), 1)
+    e = (c.dout[0, :, 0].double() * (out.double().cpu() - r["out"][0, :, 0])).sum(1)
+    given = (scale * e[:, None] * (p @ K)).norm()
+    for n, x in zip(("dq", "dk", "dv"), g):
+        w = r[n]
+        once = (w.to(dtype).double() - w).norm()
+        err = (x.view(w.shape).double().cpu() - w).norm()
+        most = 1.06 * torch.hypot(once, given) if n == "dq" else 1.5 * once
+        print(n, float(err / once), float(most / once), flush=True)
+        assert err <= most, n
