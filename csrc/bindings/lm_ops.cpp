@@ -6,6 +6,8 @@
 #include <torch/extension.h>
 #include <ATen/hip/HIPContext.h>
 #include <hip/hip_runtime.h>
+#include <algorithm>
+#include <numeric>
 #include <vector>
 
 #include "bind_util.h"
@@ -76,23 +78,49 @@ void check_cols(const torch::Tensor& t, const torch::Tensor& ref, long long off,
   if (write)
     TORCH_CHECK(B == 1 || bs >= (S - 1) * rs + W || (bs >= W && rs >= (B - 1) * bs + W), n, ": tokens overlap");
 }
-// Two column views share no element: disjoint byte ranges, or the same token stride and disjoint columns.
+// Two column views share no element.
 struct View {
   const char* at;
-  long long rs, last;  // bytes: token stride, from the first to behind the last element
-  long long w;
+  long long B, S, bs, rs, w;  // batches of tokens of w bytes, bs and rs bytes apart
   const char* n;
+  long long last() const { return (B - 1) * bs + (S - 1) * rs + w; }  // behind the last element
 };
 View view_of(const torch::Tensor& t, long long off, long long bs, long long rs, long long B, long long S, long long W, const char* n) {
-  return {(const char*)t.data_ptr() + 2 * off, 2 * rs, 2 * ((B - 1) * bs + (S - 1) * rs + W), 2 * W, n};
+  if (B > 1 && bs == S * rs) return {(const char*)t.data_ptr() + 2 * off, 1, B * S, 0, 2 * rs, 2 * W, n};  // one run of tokens
+  return {(const char*)t.data_ptr() + 2 * off, B, S, 2 * bs, 2 * rs, 2 * W, n};
 }
-void disjoint(const View& a, const View& b) {
-  const bool apart = a.at + a.last <= b.at || b.at + b.last <= a.at;
-  if (apart) return;
+long long floor_div(long long a, long long b) { return a / b - (a % b < 0 ? 1 : 0); }
+bool share(const View& a, const View& b) {
   const View &lo = a.at <= b.at ? a : b, &hi = a.at <= b.at ? b : a;
-  const long long d = a.rs == b.rs && a.rs > 0 ? (hi.at - lo.at) % a.rs : 0;
-  TORCH_CHECK(d >= lo.w && d + hi.w <= a.rs, a.n, " overlaps ", b.n);
+  const long long d = hi.at - lo.at;
+  if (d >= lo.last()) return false;
+  // modulo a divisor of all strides a view is one piece: disjoint pieces (columns of one buffer) share nothing
+  long long g = 0;
+  for (const View* v : {&lo, &hi}) {
+    if (v->B > 1) g = std::gcd(g, v->bs);
+    if (v->S > 1) g = std::gcd(g, v->rs);
+  }
+  if (g > 0 && d % g >= lo.w && d % g + hi.w <= g) return false;
+  // equal token strides: for each pair of batches, the tokens i of lo and j of hi with |overlap| > 0 are those
+  // whose i - j = m lies in [m0, m1]. (Other strides: taken to share.)
+  const long long rs = lo.S > 1 ? lo.rs : hi.S > 1 ? hi.rs : std::max(lo.w, hi.w) + d;
+  if ((lo.S > 1 && lo.rs != rs) || (hi.S > 1 && hi.rs != rs) || rs <= 0) return true;
+  const auto meet = [&](long long x) {  // x: from a batch of lo to one of hi
+    const long long m0 = std::max(floor_div(x - lo.w, rs) + 1, 1 - hi.S), m1 = std::min(floor_div(x + hi.w - 1, rs), lo.S - 1);
+    return m0 <= m1;
+  };
+  if (lo.B * hi.B > 1 << 22 && lo.bs != hi.bs) return true;
+  if (lo.bs == hi.bs) {
+    for (long long n = 1 - hi.B; n < lo.B; ++n)
+      if (meet(d - n * lo.bs)) return true;
+    return false;
+  }
+  for (long long i = 0; i < lo.B; ++i)
+    for (long long j = 0; j < hi.B; ++j)
+      if (meet(d - i * lo.bs + j * hi.bs)) return true;
+  return false;
 }
+void disjoint(const View& a, const View& b) { TORCH_CHECK(!share(a, b), a.n, " overlaps ", b.n); }
 void check_shape(const std::vector<int64_t>& s, double scale, double cap, double p_drop) {
   TORCH_CHECK(s.size() == 6, "attention shape [B,H,Hk,Sq,Sk,D]");
   for (auto v : s) TORCH_CHECK(v >= 1 && v <= 0x7fffffff, "bad attention shape");

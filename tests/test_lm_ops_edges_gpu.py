@@ -158,3 +158,35 @@ def test_attention_gradients_under_steep_slopes(slope, dtype):
         most = 1.06 * torch.hypot(once, given) if n == "dq" else 1.5 * once
         print(n, float(err / once), float(most / once), flush=True)
         assert err <= most, n
+
+
+# ------------------------------------------------------------------------------------- gradients in interleaved buffers
+
+def _grads(sp, out, lse, dout, views):
+    TR.attention_bwd(sp, out, dout, lse, *((v, 0) for v in views))
+    return [v.clone() for v in views]
+
+
+def test_attention_gradients_in_interleaved_buffers():
+    """Gradient views that share memory are refused before a launch, whatever their batch strides; views of one
+    buffer that do not share any are written (batches between the tokens, batches any distance apart)."""
+    B, S, W = 4, 8, 64
+    c = Case(B=B, H=1, Sq=S, cap=3.0, fused=False)
+    sp = c.spec()
+    out, lse = TR.attention_fwd(sp)
+    dout = c.dout.reshape(B * S, W).to(DEV)
+    want = _grads(sp, out, lse, dout, [torch.empty(B, S, W, dtype=BF, device=DEV) for _ in range(3)])
+    buf = torch.zeros(16384, dtype=BF, device=DEV)
+    view = lambda bs, rs, at: torch.as_strided(buf, (B, S, W), (bs, rs, 1), at)  # noqa: E731
+    for strides in ([(128, 1024, 0), (192, 1024, 64), (64, 1024, 768)],  # the third batch of dq is the second of dk
+                    [(1024, 128, 0), (1032, 128, 64), (1024, 128, 8192)],
+                    [(512, 64, 0), (512, 64, 2048), (512, 64, 4032)]):
+        with pytest.raises(RuntimeError, match="overlaps"):
+            _grads(sp, out, lse, dout, [view(*s) for s in strides])
+    assert not buf.any()
+    for strides in ([(192, 768, 0), (192, 768, 64), (192, 768, 128)],  # [S, B, 3 W]
+                    [(1544, 192, 0), (1544, 192, 64), (1544, 192, 128)],  # [B, S, 3 W], 8 elements between the batches
+                    [(64, 1024, 0), (128, 1024, 256), (64, 1024, 704)],
+                    [(512, 64, 0), (512, 64, 2048), (512, 64, 4096)]):
+        got = _grads(sp, out, lse, dout, [view(*s) for s in strides])
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), strides
