@@ -339,7 +339,8 @@ class AttnSpec:
     no key has output 0, lse +inf and no gradient. Keys that no query of the call sees (beyond kv_len,
     padding, other documents) may hold anything; a non-finite value in a key that some queries see can
     reach the others of the same tile. Buffers may be 2-D [B*S, width] or 3-D [B, S', width]
-    with S' >= S (a cache with room), rows any multiple of 8 elements apart."""
+    with S' >= S (a cache with room; it takes the shaped kernels by itself, a contiguous one of S tokens does not),
+    rows any multiple of 8 elements apart."""
 
     def __init__(self, B, H, Sq, Sk, q, k, v, kv_len=None, causal=False, p_drop=0.0, seed=0, scale=None, *,
                  kv_heads=None, head_dim=HEAD_DIM, softcap=0.0, slopes=None, docs=None, prefix_len=None,
@@ -351,9 +352,12 @@ class AttnSpec:
         self.scale = scale if scale is not None else 1.0 / math.sqrt(head_dim)
         self.softcap, self.slopes, self.docs = float(softcap or 0.0), slopes, docs
         self.prefix_len, self.q_start = prefix_len, q_start
+        # (f16 operands of a call without any of the arguments: the kernels of the plain form have bf16 only, its
+        # CPU reference takes any type)
         self.shaped = (self.softcap != 0.0 or slopes is not None or docs is not None or prefix_len is not None
                        or q_start is not None or self.kv_heads != H or head_dim != HEAD_DIM
-                       or q[0].dtype == torch.float16 or any(b.dim() == 3 for b, _ in (q, k, v)))
+                       or (q[0].dtype == torch.float16 and (q[0].is_cuda or kv_heads is not None))
+                       or any(b.dim() == 3 and _is_cache(b, B, S) for (b, _), S in ((q, Sq), (k, Sk), (v, Sk))))
         if self.shaped:
             self._check()
 
@@ -388,6 +392,12 @@ class AttnSpec:
             rs = buf.shape[-1]
             out += [S * rs, rs]
         return out
+
+
+def _is_cache(buf, B, S):
+    """A 3-D buffer [B, S', width] that the plain form cannot read: room behind S tokens, or batches apart."""
+    return (buf.dtype in (torch.bfloat16, torch.float16) and buf.shape[0] == B and buf.shape[1] >= S
+            and not (buf.shape[1] == S and buf.is_contiguous()))
 
 
 def _span_check(n, buf, col, B, S, W):

@@ -48,3 +48,27 @@ def test_attention_refuses_what_float32_does_not_hold(kw):
     q = randn(16, 128)
     with pytest.raises(ValueError):
         TR.AttnSpec(2, 2, 8, 8, (q, 0), (q, 0), (q, 0), **kw)
+
+
+def test_plain_3d_buffers_and_types_keep_the_plain_form():
+    """Without the new arguments contiguous [B, S, width] buffers and, on the CPU, any type are the plain form: its
+    results, its types, its arguments (a negative scale, a kv_len of more than B)."""
+    x = randn(2 * 8, 384)
+    want = TR.attention_fwd(TR.AttnSpec(2, 2, 8, 8, (x, 0), (x, 128), (x, 256), causal=True, scale=-0.1))
+    for dt in (torch.bfloat16, torch.float16, torch.float32):
+        for buf in (x.to(dt), x.to(dt).view(2, 8, 384)):
+            sp = TR.AttnSpec(2, 2, 8, 8, (buf, 0), (buf, 128), (buf, 256), causal=True, scale=-0.1)
+            assert not sp.shaped
+            out, lse = TR.attention_fwd(sp)
+            assert out.dtype == torch.bfloat16 and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+            d = torch.empty_like(buf)
+            TR.attention_bwd(sp, out, out, lse, (d, 0), (d, 128), (d, 256))
+            assert torch.isfinite(d).all()
+    y = x.view(16, 2, 192)[:, 0, :128].contiguous().view(16, 2, 64)  # heads apart: the CPU form takes it
+    assert not TR.AttnSpec(2, 2, 8, 8, (y, 0), (y, 0), (y, 0)).shaped
+    room = torch.zeros(2, 9, 384, dtype=torch.bfloat16)
+    assert TR.AttnSpec(2, 2, 8, 8, (room, 0), (room, 128), (room, 256)).shaped
+    assert TR.AttnSpec(2, 2, 8, 8, *((room[:, :8], c) for c in (0, 128, 256))).shaped
+    h = x.half()
+    sp = TR.AttnSpec(2, 2, 8, 8, (h, 0), (h, 128), (h, 256), kv_heads=2)
+    assert sp.shaped and TR.attention_fwd(sp)[0].dtype == torch.float16

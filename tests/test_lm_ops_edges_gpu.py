@@ -190,3 +190,21 @@ def test_attention_gradients_in_interleaved_buffers():
                     [(512, 64, 0), (512, 64, 2048), (512, 64, 4096)]):
         got = _grads(sp, out, lse, dout, [view(*s) for s in strides])
         assert all(torch.equal(a, b) for a, b in zip(got, want)), strides
+
+
+# ------------------------------------------------------------------------------------- plain calls keep their kernels
+
+def test_attention_plain_3d_buffers_keep_the_plain_kernels():
+    """bf16 buffers [B, S, width] of exactly S tokens are the plain form, as 2-D ones are: equal bits, its rules."""
+    B, H, S = 2, 2, 40
+    x = randn(B * S, 3 * H * 64, seed=3).to(DEV)
+    kv_len = i32([40, 7, 1]).to(DEV)  # (the plain form reads the first B)
+    res = []
+    for buf in (x, x.view(B, S, -1)):
+        sp = TR.AttnSpec(B, H, S, S, (buf, 0), (buf, H * 64), (buf, 2 * H * 64), causal=True, kv_len=kv_len)
+        assert not sp.shaped
+        out, lse = TR.attention_fwd(sp)
+        d = torch.empty_like(buf)
+        TR.attention_bwd(sp, out, out, lse, (d, 0), (d, H * 64), (d, 2 * H * 64))
+        res.append((out, lse, d.view(B * S, -1)))
+    assert all(torch.equal(a, b) for a, b in zip(*res))
