@@ -63,7 +63,7 @@ class TokenLogprobs(NamedTuple):
 TOP_K_MAX = 32
 
 
-def _logprob_args(logits, ids, V, top_k):
+def _logprob_args(logits, ids, V, top_k, ignore_index):
     if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"token_logprobs: logits must be [T, V] bf16 / f16 / f32, got {logits.dtype} {tuple(logits.shape)}")
     V = logits.shape[1] if V is None else V
@@ -75,7 +75,8 @@ def _logprob_args(logits, ids, V, top_k):
         raise ValueError(f"token_logprobs: ids must be int32 [{logits.shape[0]}], got {ids.dtype} {tuple(ids.shape)}")
     if logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError("token_logprobs: logits need unit stride along the classes")
-    return V, ids.reshape(-1).contiguous()
+    # an ignore_index that no int32 id can equal ignores nothing (-1 is outside [0, V) already)
+    return V, ids.reshape(-1).contiguous(), ignore_index if -2 ** 31 <= ignore_index < 2 ** 31 else -1
 
 
 def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, V: int | None = None, top_k: int = 0,
@@ -85,7 +86,7 @@ def token_logprobs(logits: torch.Tensor, ids: torch.Tensor, V: int | None = None
     stride apart; columns from V on are padding). ids equal to ignore_index or outside [0, V) have logp 0
     (their entropy and alternatives are computed all the same). -inf logits are classes of probability 0; a
     row of nothing else has logp -inf, entropy 0. NaN or +inf in a row make its results NaN."""
-    V, ids = _logprob_args(logits, ids, V, top_k)
+    V, ids, ignore_index = _logprob_args(logits, ids, V, top_k, ignore_index)
     if not on_gpu(logits):
         x = logits[:, :V].float()
         m = x.amax(1, keepdim=True)
@@ -116,7 +117,7 @@ def token_logprobs_bwd(logits: torch.Tensor, ids: torch.Tensor, saved: TokenLogp
         if saved.top_ids is None or dtop.shape != saved.top_ids.shape:
             raise ValueError("token_logprobs_bwd: dtop needs the alternatives of token_logprobs(top_k=...), same shape")
         k = dtop.shape[1]
-    V, ids = _logprob_args(logits, ids, V, k)
+    V, ids, ignore_index = _logprob_args(logits, ids, V, k, ignore_index)
     T, cols = logits.shape
     for n, g, shape in (("dlogp", dlogp, (T,)), ("dentropy", dentropy, (T,)), ("dtop", dtop, (T, k))):
         if g is not None and (g.dtype != torch.float32 or tuple(g.shape) != shape):

@@ -72,3 +72,13 @@ def test_plain_3d_buffers_and_types_keep_the_plain_form():
     h = x.half()
     sp = TR.AttnSpec(2, 2, 8, 8, (h, 0), (h, 128), (h, 256), kv_heads=2)
     assert sp.shaped and TR.attention_fwd(sp)[0].dtype == torch.float16
+
+
+@pytest.mark.parametrize("ignore", [2 ** 32 + 5, -2 ** 40 + 7, 2 ** 33])
+def test_logprobs_ignore_index_outside_int32(ignore):
+    """(modulo 2^32 these are 5, 7 and 0)"""
+    x, ids = randn(4, 50, dtype=torch.float32), i32([5, 5, 7, 0])
+    w, r = L.token_logprobs(x, ids), L.token_logprobs(x, ids, ignore_index=ignore)
+    assert torch.equal(r.logp, w.logp) and r.logp.all()
+    g = torch.ones(4)
+    assert torch.equal(L.token_logprobs_bwd(x, ids, r, g, ignore_index=ignore), L.token_logprobs_bwd(x, ids, w, g))

@@ -208,3 +208,16 @@ def test_attention_plain_3d_buffers_keep_the_plain_kernels():
         TR.attention_bwd(sp, out, out, lse, (d, 0), (d, H * 64), (d, 2 * H * 64))
         res.append((out, lse, d.view(B * S, -1)))
     assert all(torch.equal(a, b) for a, b in zip(*res))
+
+
+# ------------------------------------------------------------------------------------- ids and limits
+
+def test_logprobs_ignore_index_outside_int32():
+    """An ignore_index that no int32 id can equal ignores nothing."""
+    x, ids = randn(4, 50, dtype=F32).to(DEV), i32([5, 5, 7, 0]).to(DEV)
+    w = L.token_logprobs(x, ids)
+    for ignore in (2 ** 32 + 5, -2 ** 40 + 7, 2 ** 33):
+        r = L.token_logprobs(x, ids, ignore_index=ignore)
+        assert torch.equal(r.logp, w.logp)
+        g = torch.ones(4, device=DEV)
+        assert torch.equal(L.token_logprobs_bwd(x, ids, r, g, ignore_index=ignore), L.token_logprobs_bwd(x, ids, w, g))
