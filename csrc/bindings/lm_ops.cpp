@@ -128,7 +128,10 @@ void check_shape(const std::vector<int64_t>& s, double scale, double cap, double
   TORCH_CHECK(s[5] == 64 || s[5] == 128, "head dim must be 64 or 128, got ", s[5]);
   // query rows padded to whole tiles (of up to 256); block counts and row indices are 32-bit
   TORCH_CHECK(s[0] * s[1] <= 0x7fffffff && (s[3] + 256) * (s[1] / s[2]) <= 0x3fffffff && s[4] <= 0x7ffffff, "attention shape too large");
-  TORCH_CHECK(((s[3] + 256) / 32 * (s[1] / s[2]) + s[4] / 64 + 2) * s[0] * s[2] <= 0x7fffffff, "attention grid too large");
+  // threads of a launch are below 2^32 (beyond, their count wraps without an error): 2 a padded row of queries or keys
+  // and 512 blocks' shares of keys, or 512 a key head of a batch and 1024 blocks' shares where there are few rows
+  const long long inst = s[0] * s[2], rows = s[1] / s[2] * (s[3] + 256) + 256, keys = s[4] + 256;
+  TORCH_CHECK(2 * inst * std::max(rows, keys) + 512 * 512 <= 0xffffffffll && 512 * (inst + 1024) <= 0xffffffffll, "attention grid too large");
   // (within float32's whole-digit range)
   TORCH_CHECK(scale >= 1.2e-38 && scale <= 2e38, "scale must be positive, got ", scale);
   TORCH_CHECK(cap == 0.0 || (cap >= 1.2e-38 && cap <= 2e38), "softcap must be >= 0, got ", cap);
@@ -256,8 +259,7 @@ int check_logits(const torch::Tensor& x, const torch::Tensor& ids, int64_t V, in
   TORCH_CHECK(x.dim() == 2 && (x.size(1) == 1 || x.stride(1) == 1), "logits must be [T, V] with unit column stride");
   TORCH_CHECK(V >= 1 && V <= x.size(1) && x.size(1) <= 0x3fffffff, "logits: ", V, " classes of ", x.size(1), " columns");
   TORCH_CHECK(k >= 0 && k <= tfk_logprobs_kmax() && k <= V, "top_k must be in 0..min(", tfk_logprobs_kmax(), ", V), got ", k);
-  // blocks of a launch: rows times the parts of a row (512 16-byte vectors each, few rows: up to 256 blocks)
-  TORCH_CHECK(x.size(0) <= 0x7fffffff && x.size(0) * ((x.size(1) >> 11) + 1) <= 0x7fffffff, "too many rows");
+  TORCH_CHECK(x.size(0) <= 0x7fffffff, "too many rows");
   need_vec(ids, at::kInt, x.size(0), x, "ids");
   return dt;
 }

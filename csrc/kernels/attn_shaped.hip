@@ -112,7 +112,11 @@ int tfk_shaped_bwd(const void* q, const void* k, const void* v, const void* o, c
 }
 int tfk_doc_spans(const int* ids, long long B, int S, int* out, hipStream_t s) {
   if (B <= 0 || S <= 0) return 0;
-  hipLaunchKernelGGL(doc_spans_kernel, dim3((unsigned)B), dim3(DT), 0, s, ids, S, (int2*)out);
-  return hipGetLastError() == hipSuccess ? 0 : -1;
+  const long long step = 1 << 21;  // rows of a launch: below 2^32 threads (beyond, their count wraps without an error)
+  for (long long b = 0; b < B; b += step) {
+    hipLaunchKernelGGL(doc_spans_kernel, dim3((unsigned)std::min(step, B - b)), dim3(DT), 0, s, ids + b * S, S, (int2*)out + b * S);
+    if (hipGetLastError() != hipSuccess) return -1;
+  }
+  return 0;
 }
 }

@@ -14,6 +14,7 @@
 // (they find their rows by a search in `keys`), so the table is written once. Bound by that write and the read
 // of dy: order and gradient of 8192 tokens, W 1024, V 33792 bf16 45 us (155 MB, 3.5 TB/s; the write alone 21),
 // of 65536 tokens, W 768, V 131072 135 us (503 MB, 3.7 TB/s). Each further launch costs 3 to 6 us of it.
+#include <algorithm>
 #include "common.h"
 
 namespace {
@@ -247,7 +248,7 @@ __device__ __forceinline__ int lower_wave(const int* keys, int n, int k) {
 }
 
 // lpc lanes share a chunk (8 columns each, `slabs` groups across a row); blocks from `sumb` on zero
-// the rows without tokens, ZROWS rows a block. A group loads BATCH rows at once, then adds them in order:
+// the rows without tokens, from zrow on, ZROWS rows a block. A group loads BATCH rows at once, then adds them in order:
 // one row's latency at a time was most of a short batch's 18 us.
 constexpr int BATCH = 8;
 constexpr int ZROWS = 8;  // of a zeroing block: many short blocks (V 33792, W 1024: 8 36.7 us, 16 37.6, 32 38.1, 64 38.8)
@@ -255,14 +256,14 @@ template <typename T, bool ACC>
 __global__ __launch_bounds__(NT) void emb_sum_kernel(const int* __restrict__ keys, const int* __restrict__ perm, int n,
                                                      int V, int W, const T* __restrict__ dy, long long ldy,
                                                      float* __restrict__ dword, float* __restrict__ part, float scale,
-                                                     int chunk_len, int lpc, int slabs, int sumb) {
+                                                     int chunk_len, int lpc, int slabs, int sumb, int zrow) {
   if ((int)blockIdx.x >= sumb) {
     __shared__ unsigned has;
     __shared__ int range[2];
-    const int r0 = ((int)blockIdx.x - sumb) * ZROWS, nr = min(ZROWS, V - r0);
+    const int r0 = zrow + ((int)blockIdx.x - sumb) * ZROWS, nr = min(ZROWS, V - r0);
     if (threadIdx.x == 0) has = 0;
     if (threadIdx.x < 128) {
-      const int w = threadIdx.x >> 6, p = lower_wave(keys, n, r0 + w * ZROWS);
+      const int w = threadIdx.x >> 6, p = lower_wave(keys, n, r0 + w * nr);
       if ((threadIdx.x & 63) == 0) range[w] = p;
     }
     __syncthreads();
@@ -385,10 +386,15 @@ void emb_sum_launch(const int* keys, const int* perm, int n, int V, int W, const
                     float* part, float scale, int acc, hipStream_t s) {
   const int lpc = lanes_per_chunk(W), slabs = (W / 8 + lpc - 1) / lpc, cl = chunk_of(n);
   const long long chunks = ((long long)n + cl - 1) / cl;
-  const int sumb = (int)((chunks * slabs * lpc + NT - 1) / NT), zerob = acc ? 0 : (V + ZROWS - 1) / ZROWS;
+  const int sumb = (int)((chunks * slabs * lpc + NT - 1) / NT), zerob = acc ? 0 : V / ZROWS + (V % ZROWS != 0);
   if (sumb + zerob == 0) return;
-  if (acc) hipLaunchKernelGGL((emb_sum_kernel<T, true>), dim3(sumb), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb);
-  else hipLaunchKernelGGL((emb_sum_kernel<T, false>), dim3(sumb + zerob), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb);
+  // (sumb has at most 2^31 threads; a launch has below 2^32, beyond, their count wraps without an error)
+  constexpr int ZMAX = 1 << 22;
+  const int z = std::min(zerob, ZMAX);
+  if (acc) hipLaunchKernelGGL((emb_sum_kernel<T, true>), dim3(sumb), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb, 0);
+  else hipLaunchKernelGGL((emb_sum_kernel<T, false>), dim3(sumb + z), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, sumb, 0);
+  for (int z0 = z; z0 < zerob; z0 += ZMAX)
+    hipLaunchKernelGGL((emb_sum_kernel<T, false>), dim3(std::min(ZMAX, zerob - z0)), dim3(NT), 0, s, keys, perm, n, V, W, (const T*)dy, ldy, dword, part, scale, cl, lpc, slabs, 0, z0 * ZROWS);
   if (chunks < 2) return;
   const dim3 g((unsigned)(chunks - 1), slabs);
   if (acc) hipLaunchKernelGGL(emb_join_kernel<true>, g, dim3(NT), 0, s, keys, n, V, W, part, dword, scale, cl, lpc);

@@ -424,6 +424,8 @@ void cut(int vecs, long long T, int nv, int& parts, int& per) {
   parts = (int)std::max(least, std::min(most, 256 / std::max(T, 1ll)));
   per = (vecs + parts - 1) / parts;
 }
+// A launch has below 2^32 threads (beyond, the count wraps without an error): rows go out in slices of at most 2^23 blocks
+constexpr int SLICE = 1 << 23;
 int vecs_of(int cols, int dtype) { const int n = dtype == 2 ? 4 : 8; return (cols + n - 1) / n; }
 }  // namespace
 
@@ -443,15 +445,24 @@ int tfk_logprobs_fwd(const void* x, int dtype, const int* ids, int T, int V, lon
   cut(vecs_of(V, dtype), T, NV, p.parts, p.per);
   p.pkeys = (u64*)ws;
   p.pstat = (Stat*)((u64*)ws + (long long)T * p.parts * k);
-  const dim3 g((unsigned)((long long)T * p.parts));
+  const int step = SLICE / p.parts;
 #define TFK_LP(T_)                                                                                              \
   if (k) hipLaunchKernelGGL((logprobs_fwd_kernel<T_, true>), g, dim3(NT), 0, s, p);                             \
   else hipLaunchKernelGGL((logprobs_fwd_kernel<T_, false>), g, dim3(NT), 0, s, p);                              \
-  if (p.parts > 1 && k) hipLaunchKernelGGL((logprobs_join_kernel<T_, true>), dim3(T), dim3(NT), 0, s, p);       \
-  else if (p.parts > 1) hipLaunchKernelGGL((logprobs_join_kernel<T_, false>), dim3(T), dim3(64), 0, s, p);
-  if (dtype == 0) { TFK_LP(bf16) } else if (dtype == 1) { TFK_LP(f16) } else { TFK_LP(float) }
+  if (p.parts > 1 && k) hipLaunchKernelGGL((logprobs_join_kernel<T_, true>), dim3(p.T), dim3(NT), 0, s, p);     \
+  else if (p.parts > 1) hipLaunchKernelGGL((logprobs_join_kernel<T_, false>), dim3(p.T), dim3(64), 0, s, p);
+  for (long long r = 0; r < T; r += step) {
+    p.T = (int)std::min<long long>(step, T - r);
+    const dim3 g((unsigned)p.T * p.parts);
+    if (dtype == 0) { TFK_LP(bf16) } else if (dtype == 1) { TFK_LP(f16) } else { TFK_LP(float) }
+    if (hipGetLastError() != hipSuccess) return -1;
+    p.x = (const char*)p.x + step * ld * (dtype == 2 ? 4 : 2);
+    p.ids += step; p.logp += step; p.ent += step; p.lse += step; p.norm += 2ll * step;
+    if (k) { p.top_logp += (long long)step * k; p.top_ids += (long long)step * k; }
+    p.pkeys += (long long)step * p.parts * k; p.pstat += (long long)step * p.parts;
+  }
 #undef TFK_LP
-  return hipGetLastError() == hipSuccess ? 0 : -1;
+  return 0;
 }
 // dx: cols >= V columns, row stride ldd; dlogp / dent may be null; k = 0: no alternatives
 int tfk_logprobs_bwd(const void* x, int dtype, const int* ids, int T, int V, long long ld, int k, int ignore,
@@ -460,10 +471,22 @@ int tfk_logprobs_bwd(const void* x, int dtype, const int* ids, int T, int V, lon
   if (T <= 0) return 0;
   BwdParams p{x, dx, ids, top_ids, ld, ldd, V, T, k, ignore, 0, 0, cols, norm, ent, dlogp, dent, dtop};
   cut(vecs_of(cols, dtype), T, BNV, p.parts, p.per);
-  const dim3 g((unsigned)((long long)T * p.parts));
-  if (dtype == 0) hipLaunchKernelGGL(logprobs_bwd_kernel<bf16>, g, dim3(NT), 0, s, p);
-  else if (dtype == 1) hipLaunchKernelGGL(logprobs_bwd_kernel<f16>, g, dim3(NT), 0, s, p);
-  else hipLaunchKernelGGL(logprobs_bwd_kernel<float>, g, dim3(NT), 0, s, p);
-  return hipGetLastError() == hipSuccess ? 0 : -1;
+  const int step = SLICE / p.parts;
+  for (long long r = 0; r < T; r += step) {
+    p.T = (int)std::min<long long>(step, T - r);
+    const dim3 g((unsigned)p.T * p.parts);
+    if (dtype == 0) hipLaunchKernelGGL(logprobs_bwd_kernel<bf16>, g, dim3(NT), 0, s, p);
+    else if (dtype == 1) hipLaunchKernelGGL(logprobs_bwd_kernel<f16>, g, dim3(NT), 0, s, p);
+    else hipLaunchKernelGGL(logprobs_bwd_kernel<float>, g, dim3(NT), 0, s, p);
+    if (hipGetLastError() != hipSuccess) return -1;
+    const int e = dtype == 2 ? 4 : 2;
+    p.x = (const char*)p.x + step * ld * e;
+    p.dx = (char*)p.dx + step * ldd * e;
+    p.ids += step; p.norm += 2ll * step; p.ent += step;
+    if (p.dlogp) p.dlogp += step;
+    if (p.dent) p.dent += step;
+    if (k) { p.top_ids += (long long)step * k; p.dtop += (long long)step * k; }
+  }
+  return 0;
 }
 }

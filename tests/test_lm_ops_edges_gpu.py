@@ -221,3 +221,46 @@ def test_logprobs_ignore_index_outside_int32():
         assert torch.equal(r.logp, w.logp)
         g = torch.ones(4, device=DEV)
         assert torch.equal(L.token_logprobs_bwd(x, ids, r, g, ignore_index=ignore), L.token_logprobs_bwd(x, ids, w, g))
+
+
+# (a launch has below 2^32 threads; beyond, their count wraps and no error is reported)
+
+def test_logprobs_of_many_rows():
+    T, V = (1 << 24) + 1000, 3
+    x = torch.randn(T, V, generator=torch.Generator(DEV).manual_seed(1), device=DEV).to(BF)
+    ids = torch.randint(0, V, (T,), generator=torch.Generator(DEV).manual_seed(2), device=DEV, dtype=torch.int32)
+    g = [torch.randn(T, generator=torch.Generator(DEV).manual_seed(3 + i), device=DEV) for i in range(2)]
+    g.append(torch.randn(T, 2, generator=torch.Generator(DEV).manual_seed(5), device=DEV))
+    r = L.token_logprobs(x, ids, top_k=2)
+    d = L.token_logprobs_bwd(x, ids, r, *g)
+    for at in (0, 999, (1 << 23) - 50, (1 << 24) - 50, T - 100):
+        s = slice(at, at + 100)
+        w = L.token_logprobs(x[s], ids[s], top_k=2)
+        for n in ("logp", "entropy", "lse", "norm", "top_logp", "top_ids"):
+            assert torch.equal(getattr(r, n)[s], getattr(w, n)), (n, at)
+        assert torch.equal(d[s], L.token_logprobs_bwd(x[s], ids[s], w, *(t[s] for t in g))), at
+    # every row, against the definition: a few roundings of exponents and logarithms of size 10
+    want = torch.log_softmax(x.float(), 1).gather(1, ids.long()[:, None])[:, 0]
+    assert float((r.logp - want).abs().max()) < 20 * 2.0 ** -23
+
+
+def test_document_spans_of_many_rows():
+    B = (1 << 22) + 5
+    ids = torch.randint(-1, 2, (B, 3), generator=torch.Generator().manual_seed(1), dtype=torch.int32)
+    assert torch.equal(TR.document_spans(ids.to(DEV)).cpu(), TR.document_spans(ids))
+
+
+def test_sorted_embedding_of_a_table_of_many_rows():
+    V = (1 << 27) + 67
+    at = [0, 8, (1 << 25) - 1, 1 << 25, (1 << 25) + 8, 1 << 26, (1 << 27) - 1, V - 4, V - 1]
+    dw = torch.full((V, 8), math.nan, device=DEV)
+    TR.embedding_bwd_sorted(TR.token_order(i32(at + [-1, V]).to(DEV), V), torch.ones(len(at) + 2, 8, dtype=BF, device=DEV), dw, accumulate=False)
+    assert torch.equal(torch.nonzero(dw[:, 3])[:, 0].cpu(), torch.tensor(at))
+    assert dw.sum().item() == 8 * len(at)
+
+
+def test_attention_refuses_grids_past_32_bits():
+    e = lambda B, S: torch.empty(1, 1, 64, dtype=BF, device=DEV).expand(B, S, 64)  # noqa: E731
+    for B, Sq, Sk in ((9_000_000, 1, 1), (8_000_000, 1, 40), (100_000, 30_000, 1)):
+        with pytest.raises(RuntimeError, match="grid too large"):
+            TR.attention_fwd(TR.AttnSpec(B, 1, Sq, Sk, (e(B, Sq), 0), (e(B, Sk), 0), (e(B, Sk), 0), softcap=1.0))
