@@ -49,7 +49,6 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // streamed rows of a tile
 constexpr int key_tile(int D) { return 64; }    // forward, dQ
 constexpr int query_tile(int D) { return 64; }  // dK/dV
-constexpr float RAISE = 8.f;  // log2 units by which a row may outgrow its running maximum
 
 template <typename T>
 struct Ty;
@@ -62,7 +61,7 @@ struct Ty<bf16> {
   }
   static __device__ __forceinline__ x4 tr(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS x4*)p); }
   static constexpr bool fits = true;  // has float's exponents
-  static constexpr float p_up = 0.f;
+  static constexpr float p_up = 0.f, raise = 8.f;
 };
 template <>
 struct Ty<f16> {
@@ -75,7 +74,7 @@ struct Ty<f16> {
     return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p));
   }
   static constexpr bool fits = false;   // 2^-14 .. 2^16
-  static constexpr float p_up = 15.f;   // log2 of the factor that the dK/dV pass gives P <= 1: whole digits down to 2^-29
+  static constexpr float p_up = 15.f, raise = 3.f;
 };
 
 struct Shaped {
@@ -291,9 +290,13 @@ __device__ __forceinline__ typename Ty<T>::x8 pack8(const f32x16& a, int half) {
   return r;
 }
 
-// f16 operands of the gradient products. dS = P (dP - delta) (1 - t^2) goes with 1 / keys and with the upstream gradient:
-// unscaled it left f16's range on long rows, for gradients of 1e-3 and smaller (no digits) and of 1e4 (infinite). So a
-// lane's row (dQ) or key (dK) has a power of two `up` for its dS, divided out of the f32 sums at the end: from 2^START,
+// f16 operands. P <= 1 goes into its products times 2^p_up, so it has whole digits down to 2^-29 (unscaled: 2^-14, and a
+// row that gives most of its weight to one key with a small V lost the rest: 16384 keys that share 1%, O off by 0.010
+// of itself, now 0.0003). The forward's P may pass 1 by 2^raise, the log2 units by which a row may outgrow its running
+// maximum before it is rescaled.
+// dS = P (dP - delta) (1 - t^2) goes with 1 / keys and with the upstream gradient: unscaled it left f16's range on long
+// rows, for gradients of 1e-3 and smaller (no digits) and of 1e4 (infinite). So a lane's row (dQ) or key (dK) has a
+// power of two `up` for its dS, divided out of the f32 sums at the end: from 2^START,
 // too large for nearly any row, it falls where an element of the row would pass 2^15, to 2^12 .. 2^13 for that element, and
 // the sums so far fall with it. The largest |dS| of a lane's row or key so far is then above 2^12, and what lies 2^26
 // below it keeps all its digits. It costs an f16 backward 5 to 11% (B1 H16/4 S8192 D128 capped 1089 -> 1143 us, B2 H16

@@ -73,6 +73,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
   constexpr bool drop = O::drop;
   const uint32_t hs = drop ? head_seed(p, b * p.H + head) : 0u;
   const int qg = (q >> 2) * p.Sk;
+  constexpr float RAISE = Ty<T>::raise, UP = Ty<T>::fits ? 0.f : Ty<T>::p_up - RAISE;  // P is 2^UP times itself
   float m = -INFINITY, lsum = 0.f;  // lsum: this lane's half of the row
   f32x16 o[D / 32];
 #pragma unroll
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
 #pragma unroll
           for (int e = 0; e < 16; ++e) o[db][e] *= alpha;
       }
-      const float nm = m == -INFINITY ? 0.f : -m;
+      const float nm = m == -INFINITY ? 0.f : UP - m;
       if (O::bias) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[e] = ex2(s[e] + nm);
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
         for (int u = 0; u < 4; ++u) v[u] = (T)(sees ? o[db][e + u] * inv : 0.f);
         *(typename Ty<T>::x4*)(Or + db * 32 + srow(e)) = v;
       }
-    if (h == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = sees && lsum != 0.f ? (m + sc.base + __log2f(lsum)) * LN2 : INFINITY;
+    if (h == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = sees && lsum != 0.f ? (m + sc.base + (__log2f(lsum) - UP)) * LN2 : INFINITY;
   }
 }
 
@@ -244,6 +245,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
   const float slope = slope_of<O>(p, head);
   const int pos = q + mk.shift;
   const float fs = O::cap || O::wide ? 1.f : sc.mult, fx = O::bias ? 1.f : fs;  // factors left to the bias, to the exponent
+  constexpr float UP = Ty<T>::p_up;  // P is 2^UP times itself
   float m = -INFINITY, lsum = 0.f;
   f32x16 o[D / 32];
 #pragma unroll
@@ -304,7 +306,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[kb][e] = ex2(fmaf(s[kb][e], fx, -muse));
+        s[kb][e] = ex2(fmaf(s[kb][e], fx, UP - muse));
         rs += s[kb][e];
       }
     lsum = fmaf(lsum, alpha, xor_sum<32>(rs));
@@ -383,7 +385,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
       for (int u = 0; u < 4; ++u) v[u] = (T)(sees ? o[db][e + u] * inv : 0.f);
       *(typename Ty<T>::x4*)(Or + db * 32 + srow(e)) = v;
     }
-  if (h == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = sees && L != 0.f ? (M + sc.base + __log2f(L)) * LN2 : INFINITY;
+  if (h == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = sees && L != 0.f ? (M + sc.base + (__log2f(L) - UP)) * LN2 : INFINITY;
 }
 // one wave per (instance, row): the splits' parts in order
 template <typename T, int D>
@@ -411,7 +413,7 @@ __global__ __launch_bounds__(64) void shaped_few_join_kernel(Shaped p, int split
   T* Or = (T*)p.out + b * p.o_bs + q * p.o_rs + head * D;
 #pragma unroll
   for (int u = 0; u < D / 64; ++u) Or[u * 64 + l] = (T)(o[u] * inv);
-  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + (shifted(p) ? p.cap * LOG2E : 0.f) + __log2f(L)) * LN2 : INFINITY;
+  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + (shifted(p) ? p.cap * LOG2E : 0.f) + (__log2f(L) - Ty<T>::p_up)) * LN2 : INFINITY;
 }
 
 // few rows and no dropout: the split form; shares of a cache so that there are about 4 blocks for each of

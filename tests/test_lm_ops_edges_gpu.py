@@ -87,6 +87,28 @@ def test_attention_f16_dropout(kw):
     Case(dtype=HF, **kw).check()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kw", [dict(Sq=2, H=4, Hk=2), dict(Sq=1, H=8, Hk=1, D=128, cap=50.0), dict(Sq=70, H=1), dict(Sq=66, H=2, Hk=1, D=128, cap=50.0),
+                                dict(Sq=64, H=1, slopes=1e-4)],
+                         ids=["few", "few_cap", "tiles", "tiles_cap", "tiles_bias"])
+def test_attention_weights_far_below_the_largest(kw, dtype):
+    """Each row gives 99% of its weight to one key with V = 0 and shares the rest among 16384: each of them weighs about
+    2^-21 of the largest. O is the sum over them: P and O are rounded, sqrt(2) times the error of O rounded once."""
+    c = Case(B=1, Sk=16384, dtype=dtype, fused=False, **kw)
+    gap = math.log(99 * 16384)
+    c.q[..., 0], c.k[..., 0], c.k[:, 300] = 8.0, 0.0, 0.0
+    c.k[:, 300, :, 0] = gap * math.sqrt(c.D) / 8.0  # (a cap of 50 takes 0.4 of 14.3 away)
+    c.v[:, 300] = 0.0
+    r, sp = c.oracle(False), c.spec()
+    out, lse = TR.attention_fwd(sp)
+    w = r["out"]
+    once = (w.to(dtype).double() - w).norm()
+    err = (out.view(w.shape).double().cpu() - w).norm()
+    print(float(once / w.norm()), float(err / w.norm()), flush=True)
+    assert err <= 1.5 * once
+    assert float((lse.double().cpu() - r["lse"]).abs().max()) < 2e-5 * 20
+
+
 # ------------------------------------------------------------------------------------- any score cap
 
 @pytest.mark.parametrize("cap", [1.2e-38, 1e-30, 1e-3, 128.0, 512.0, 513.0, 1e4, 1e6, 1e8, 1e30, 2e38])
