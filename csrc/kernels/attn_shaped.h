@@ -40,15 +40,12 @@ typedef _Float16 f16;
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <bool B>
 using bconst = std::integral_constant<bool, B>;
 template <int I>
 using iconst = std::integral_constant<int, I>;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-// streamed rows of a tile
-constexpr int key_tile(int D) { return 64; }    // forward, dQ
-constexpr int query_tile(int D) { return 64; }  // dK/dV
+constexpr int KT = 64;  // streamed rows of a tile: keys (forward, dQ), queries (dK/dV)
 
 template <typename T>
 struct Ty;
@@ -193,7 +190,7 @@ struct Mask {
   __device__ __forceinline__ Span of(int q) const {
     return of<DOCS>(q, DOCS ? doc_at(q + shift) : int2{0, 0});
   }
-  // positions that see key j < Sk: [lo, hi) (superset; the pair test decides)
+  // positions that see key j < Sk: [lo, hi), exactly (documents: runs of document_spans, the same at both of a pair's ends)
   template <bool DOCS>
   __device__ __forceinline__ Span seen_by(int j) const {
     Span s{-(1 << 30), 0x7fffffff};
@@ -357,7 +354,7 @@ __device__ __forceinline__ void dma_b32(__amdgpu_buffer_rsrc_t r, unsigned lds, 
   asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(voff), "s"(r) : "memory");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-template <int D, int NW, int KT>
+template <int D, int NW>
 struct Dma {
   static constexpr int N = KT * D * 2 / (NW * 1024), RPI = 512 / D, STEP = NW * RPI;
   static_assert(N >= 1 && (N == 1 || STEP % 16 == 0), "one swizzle for all instructions of a lane");
@@ -465,11 +462,11 @@ struct Reach {
 };
 // With documents: one 4-byte mark for each staged row of the lane, loaded into the wave's own LDS words
 // beside the tile; rows whose mark says that nothing sees them are cleared.
-template <int D, int NW, int KT>
+template <int D, int NW>
 struct DeadRows {
-  static constexpr int N = Dma<D, NW, KT>::N, WORDS = N * NW * 64;  // of one slot
+  static constexpr int N = Dma<D, NW>::N, WORDS = N * NW * 64;  // of one slot
   // marks at base[row * stride_b bytes + at], rows outside [0, rows) read 0
-  static __device__ __forceinline__ void issue(const void* base, int stride, int at, int rows, int row0, const Dma<D, NW, KT>& m, unsigned lds) {
+  static __device__ __forceinline__ void issue(const void* base, int stride, int at, int rows, int row0, const Dma<D, NW>& m, unsigned lds) {
     const __amdgpu_buffer_rsrc_t r = rows_rsrc(base, stride, rows);
     const int w = threadIdx.x >> 6;
 #pragma unroll

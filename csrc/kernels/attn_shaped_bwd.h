@@ -18,8 +18,8 @@ constexpr int dq_min_waves(int D, bool drop, bool fits) { return D == 64 && (fit
 template <typename T, int D, int NW, typename O>
 __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) void shaped_dq_kernel(Shaped p) {
   constexpr bool DOCS = O::docs;
-  constexpr int KT = key_tile(D), TB = KT * D * 2;
-  typedef DeadRows<D, NW, KT> Dead;
+  constexpr int TB = KT * D * 2;
+  typedef DeadRows<D, NW> Dead;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB];  // [slot][K | V]
   __shared__ __attribute__((aligned(256))) unsigned marks[DOCS ? 2 * Dead::WORDS : 1];
   __shared__ int range[2][NW];
@@ -50,7 +50,7 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
 
   const T* Kb = (const T*)p.k + b * p.k_bs + hk * D;
   const T* Vb = (const T*)p.v + b * p.v_bs + hk * D;
-  Dma<D, NW, KT> km, vm;
+  Dma<D, NW> km, vm;
   km.init(p.k_rs);
   vm.init(p.v_rs);
   auto issue = [&](int t, int slot) {
@@ -202,8 +202,8 @@ __device__ __forceinline__ float dk_scale(const Shaped& p) { return shifted(p) ?
 template <typename T, int D, int NW, typename O>
 __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv_kernel(Shaped p, int splits, float* __restrict__ part) {
   constexpr bool DOCS = O::docs;
-  constexpr int KT = query_tile(D), TB = KT * D * 2;
-  typedef DeadRows<D, NW, KT> Dead;
+  constexpr int TB = KT * D * 2;
+  typedef DeadRows<D, NW> Dead;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB + NW * 64 * D];  // [slot][Q | dO], K
   __shared__ __attribute__((aligned(256))) float stat[2][2][64];  // [slot][lse in log2 units, -delta]
   __shared__ __attribute__((aligned(256))) unsigned marks[DOCS ? 2 * Dead::WORDS : 1];
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
 
   // the wave's K rows: one address, the k-slots by XOR (8 addresses more would spill)
   int krow = fo.row[0] + 4 * TB + w * 64 * D;
-  Dma<D, NW, KT> qm, om;
+  Dma<D, NW> qm, om;
   qm.init(p.q_rs);
   om.init(p.o_rs);
   int g_next = i0 / max(nt, 1), t_next = i0 % max(nt, 1);  // (head, tile) of the next issue
@@ -273,7 +273,7 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   };
   if (i0 < i1) {
     {
-      Dma<D, NW, KT> km;
+      Dma<D, NW> km;
       km.init(p.k_rs);
       const int kb = tile * NW * 32;
 #pragma unroll

@@ -9,8 +9,8 @@ namespace {
 template <typename T, int D, int NW, typename O>
 __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Shaped p) {
   constexpr bool DOCS = O::docs;
-  constexpr int KT = key_tile(D), TB = KT * D * 2;
-  typedef DeadRows<D, NW, KT> Dead;
+  constexpr int TB = KT * D * 2;
+  typedef DeadRows<D, NW> Dead;
   __shared__ __attribute__((aligned(1024))) char smem[4 * TB];  // [slot][K | V]
   __shared__ __attribute__((aligned(256))) unsigned marks[DOCS ? 2 * Dead::WORDS : 1];
   __shared__ int range[2][NW];
@@ -41,7 +41,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
 
   const T* Kb = (const T*)p.k + b * p.k_bs + hk * D;
   const T* Vb = (const T*)p.v + b * p.v_bs + hk * D;
-  Dma<D, NW, KT> km, vm;
+  Dma<D, NW> km, vm;
   km.init(p.k_rs);
   vm.init(p.v_rs);
   auto issue = [&](int t, int slot) {

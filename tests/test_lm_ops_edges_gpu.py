@@ -286,3 +286,18 @@ def test_attention_refuses_grids_past_32_bits():
     for B, Sq, Sk in ((9_000_000, 1, 1), (8_000_000, 1, 40), (100_000, 30_000, 1)):
         with pytest.raises(RuntimeError, match="grid too large"):
             TR.attention_fwd(TR.AttnSpec(B, 1, Sq, Sk, (e(B, Sq), 0), (e(B, Sk), 0), (e(B, Sk), 0), softcap=1.0))
+
+
+# ------------------------------------------------------------------------------------- the operators' neighbours
+
+@pytest.mark.parametrize("T,V,W,scale", [(333, 4099, 512, 22.6), (8192, 3000, 768, 1.0), (20000, 40, 64, 8.0)])
+def test_sorted_embedding_agrees_with_the_bucketed_one(T, V, W, scale):
+    """Both add the same terms in float32 in an order of their own: n additions each."""
+    ids = zipf(T, V).clamp(min=0).to(DEV)
+    dy = randn(T, W, seed=2).to(DEV)
+    a, b = torch.zeros(V, W, device=DEV), torch.zeros(V, W, device=DEV)
+    TR.embedding_bwd_sorted(TR.token_order(ids, V), dy, a, scale=scale)
+    TR.embedding_bwd(ids, dy, b, scale=scale)
+    n = torch.bincount(ids.long(), minlength=V)[:, None].double().cpu()
+    mag = torch.zeros(V, W, dtype=torch.float64).index_add_(0, ids.long().cpu(), dy.double().abs().cpu()) * scale
+    O.within(a, b.double().cpu(), 2 * (n + 3) * 2.0 ** -24 * mag, "dword")
