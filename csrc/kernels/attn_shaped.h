@@ -435,14 +435,25 @@ __device__ __forceinline__ void locate(int columns, int& column, int& rank) {
   column = (int)blockIdx.x % columns;
 }
 
-// waves of 32 rows in a block of the forward and of the dQ pass. 4; at D = 128, where a CU holds 8 waves, all 8
-// in one block that reads each key tile once instead of twice, if there are 512 such blocks (B1 H16/4 S8192:
-// forward 358 -> 346 us, dQ 459 -> 417 us; with fewer blocks the longest tiles end late, and at D = 64, with 12
-// to 16 waves a CU, 8 were slower: forward 27.8 -> 30.1, dQ 35.4 -> 44.5 us for B4 H16 S2048 in documents of
-// about 512). Dropout's instances keep 4.
-__host__ __device__ constexpr int max_row_waves(int D, bool drop) { return D == 128 && !drop ? 8 : 4; }
+// waves of 32 rows in a block of the forward and of the dQ pass. 4; 8, which read each key tile once instead of twice, at
+// D = 128, where a CU holds 8 waves, if their blocks are two full rounds of the 256 CUs (449 .. 512) of 3584 queries or
+// more: blocks are long then, and every CU gets a long and a short one. Forward / backward in us, 4 -> 8 waves, causal bf16:
+//   two rounds:   S7424 H16 238 / 804 -> 225 / 792, S8192 H16 288 / 918 -> 268 / 897 (cap 30: 366 / 1074 -> 351 / 1048),
+//                 S32000 H4 1067 / 3337 -> 984 / 3252, S4096 H32 151 / 502 -> 143 / 497
+//   other counts: S4096 H16 96 / 301 -> 110 / 322, S6144 163 / 565 -> 179 / 589, S10240 426 / 1450 -> 442 / 1481 (cap 30:
+//                 535 / 1679 -> 582 / 1735), S12288 604 / 2036 -> 618 / 2060, S16384 within 3% either way
+//   short rows:   S1024 B8 H16 52 / 201 -> 54 / 208, S2048 H64 cap 30 102 / 331 -> 104 / 335
+//   documents:    S8192 H16 134 / 409 -> 140 / 411 (cap 30: 148 / 445 -> 177 / 477); cap and bias: 404 / 1175 -> 441 / 1158
+// (At D = 64, with 12 to 16 waves a CU, 8 were slower: forward 27.8 -> 30.1, dQ 35.4 -> 44.5 for B4 H16 S2048 in documents
+// of about 512.) Dropout's and wide caps' instances keep 4.
+template <typename O>
+__host__ __device__ constexpr int max_row_waves(int D) {
+  return D == 128 && !O::drop && !O::docs && !O::wide && !(O::cap && O::bias) ? 8 : 4;
+}
 inline int row_waves(const Shaped& p, int D) {
-  return max_row_waves(D, p.p_drop > 0.f) == 8 && p.B * (long long)p.H * (p.Sq / 256) >= 512 ? 8 : 4;
+  const bool has = D == 128 && p.p_drop == 0.f && !p.docs && p.cap <= CAP_SHIFT && !(p.cap > 0.f && p.slopes);
+  const long long blocks = p.B * (long long)p.H * ((p.Sq + 255) / 256);
+  return has && p.Sq >= 3584 && blocks > 448 && blocks <= 512 ? 8 : 4;
 }
 
 inline void row_tiles(Shaped& p, int rows) {

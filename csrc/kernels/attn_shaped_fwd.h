@@ -437,7 +437,7 @@ int launch_fwd(Shaped p, float* part, hipStream_t s) {
   row_tiles(p, waves * 32);
   const dim3 grid((unsigned)(p.tiles * p.heads * p.B * p.Hk)), block(waves * 64);
   with_rules(p, [&](auto o) {
-    constexpr int MAX = max_row_waves(D, decltype(o)::drop);
+    constexpr int MAX = max_row_waves<decltype(o)>(D);
     if (waves == MAX) hipLaunchKernelGGL((shaped_fwd_kernel<T, D, MAX, decltype(o)>), grid, block, 0, s, p);
     else hipLaunchKernelGGL((shaped_fwd_kernel<T, D, 4, decltype(o)>), grid, block, 0, s, p);
   });

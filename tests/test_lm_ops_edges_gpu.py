@@ -301,3 +301,28 @@ def test_sorted_embedding_agrees_with_the_bucketed_one(T, V, W, scale):
     n = torch.bincount(ids.long(), minlength=V)[:, None].double().cpu()
     mag = torch.zeros(V, W, dtype=torch.float64).index_add_(0, ids.long().cpu(), dy.double().abs().cpu()) * scale
     O.within(a, b.double().cpu(), 2 * (n + 3) * 2.0 ** -24 * mag, "dword")
+
+
+# ------------------------------------------------------------------------------------- variants by size
+
+# 449 to 512 blocks of 256 rows at head size 128: the row tiles of 8 waves; beside them, of 4
+ROWS = {
+    "causal": lambda: Case(B=1, H=32, Hk=4, D=128, Sq=3700, Sk=150, causal=True, q_start=[-3600], cap=6.0, fused=False),
+    "full_f16": lambda: Case(B=2, H=16, Hk=2, D=128, Sq=3584 + 130, Sk=97, dtype=HF, kv_len=[97, 40], poison=math.nan, fused=False),
+    "bias": lambda: Case(B=1, H=32, Hk=2, D=128, Sq=4000, Sk=90, causal=True, slopes=True, q_start=[-3950], fused=False),
+    "prefix": lambda: Case(B=1, H=30, Hk=15, D=128, Sq=3840, Sk=200, causal=True, prefix_len=[70], q_start=[-3700], fused=False),
+    "bias_cap": lambda: Case(B=1, H=32, Hk=2, D=128, Sq=3700, Sk=90, causal=True, slopes=True, cap=9.0, q_start=[-3650], fused=False),
+    "more_blocks": lambda: Case(B=1, H=34, Hk=2, D=128, Sq=4000, Sk=64, causal=True, q_start=[-3950], fused=False),
+}
+
+
+@pytest.mark.parametrize("name", list(ROWS))
+def test_attention_row_tiles(name):
+    ROWS[name]().check()
+
+
+@pytest.mark.parametrize("T", [180000, 180001])
+def test_token_order_tiles(T):
+    ids = torch.randint(-3, 33003, (T,), generator=torch.Generator().manual_seed(T), dtype=torch.int32)
+    a, b = TR.token_order(ids.to(DEV), 33000), TR.token_order(ids, 33000)
+    assert torch.equal(a.perm.cpu(), b.perm) and torch.equal(a.keys.cpu(), b.keys)
