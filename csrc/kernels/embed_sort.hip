@@ -88,10 +88,11 @@ __global__ __launch_bounds__(1024) void order_count_kernel(const int* __restrict
 constexpr int RT = 512, RW = RT / 64;  // threads, waves of a sorting block
 constexpr int RB_MAX = 10;             // digit bits
 // items of a tile (each wave: consecutive ones): small tiles for more blocks, large ones because each block reads
-// the histograms of all tiles (65536 items of 18 bits: 1024 19.1 us, 2048 21.0, 4096 27.7; 2^20 of 16 bits: 108, 60,
-// 48; 2^22 of 18 bits: 2309, 664, 262)
+// the histograms of all tiles (tiles of 1024 and 4096, us: 65536 items of 16 bits 18.5 and 23.0, 131072 22.1 and 24.1,
+// 163840 24.4 and 28.2, 196608 26.8 and 25.6, 262144 31.8 and 26.7, 2^20 108 and 48; of 18 bits: 163840 27.4 and 30.3,
+// 196608 30.5 and 27.9, 2^22 2309 and 262)
 constexpr int RTILE_FEW = 1024, RTILE_MANY = 4096;
-int radix_tile(long long T) { return T <= 131072 ? RTILE_FEW : RTILE_MANY; }
+int radix_tile(long long T) { return T <= 180000 ? RTILE_FEW : RTILE_MANY; }
 
 template <bool FIRST>
 __device__ __forceinline__ int radix_key(const int* src, long long i, int V) {
