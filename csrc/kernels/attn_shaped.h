@@ -26,10 +26,12 @@
 // LDS rows are D elements, their 16-byte chunks XOR-swizzled (swz): conflict-free for both reads.
 //
 // Bound by arithmetic: an element costs 4 D (dQ: 6 D, dK/dV: 8 D) matrix flops and 9 to 20 vector instructions
-// with one or two exponentials, and the two units overlap only between the waves of a SIMD (vector unit busy
-// 60 to 66%, matrix unit 37 to 48%). B1 H16/4 S8192 D128 bf16, causal, capped: forward 358 us (770 TFLOP/s),
-// dQ 453 us (910), dK/dV 576 us (955) and 24 us of its join. B4 H16 S2048 D64 in documents of about 512: 29, 41
-// and 53 us, half of them the exponentials and masks of tiles that a document fills in part.
+// with one or two exponentials, and the two units overlap only between the waves of a SIMD. B1 H16/4 S8192 D128 bf16,
+// causal, capped: forward 389 to 408 us (700 TFLOP/s; alone 351), dQ 477 to 505 (850), dK/dV 584 to 616 (920) and 24 of
+// its join, as the clock goes; vector unit busy 60 / 54 / 47% of the CUs' busy cycles, matrix unit 34 / 42 / 46%.
+// B4 H16 S2048 D64 in documents of about 512: 29, 41 and 53 us, vector unit 56 / 41 / 31%, matrix unit 20 / 23 / 22%: the
+// waves wait 42 to 45% of their cycles. A block walks the tiles between its rows' first and last key, of which a wave has
+// work in 74% (dK/dV works on 64 queries where 32 would do: 78% of its pairs are needed, 88% by 32).
 #pragma once
 #include <algorithm>
 #include "common.h"

@@ -417,7 +417,9 @@ __global__ __launch_bounds__(64) void shaped_few_join_kernel(Shaped p, int split
 }
 
 // few rows and no dropout: the split form; shares of a cache so that there are about 4 blocks for each of
-// 256 CUs, none below 512 keys
+// 256 CUs, none below 512 keys (one token, H32/8 D128, caches half to all full, us: B16 Sk 16384 with 2, 4 and 8 blocks a
+// CU 168, 165 and 170, Sk 65536 626, 595 and 567, B64 Sk 2048 93, 97 and 114; shares from 256, 512 and 1024 keys: B1 Sk 2048
+// 16, 18 and 20, Sk 16384 37, 26 and 24, B16 Sk 2048 44, 34 and 28, Sk 16384 equal)
 bool few_rows(int G, int Sq, float p_drop) { return G * (long long)Sq <= 32 && p_drop == 0.f; }
 int few_splits(int inst, int Sk) { return std::max(1, std::min((1024 + inst - 1) / inst, Sk / 512)); }
 template <typename T, int D>

@@ -13,8 +13,8 @@
 // NT * NV 16-byte vectors; a part lives in the registers of one block, which reduces it to (m, S, Y) and
 // its k best, and a second launch joins the parts of a row (a row of one part is finished at once).
 // So a few long rows fill the card as many short ones do. f32 sums throughout. 8192 rows of 33708 bf16 logits:
-// forward 129 us (4.3 TB/s), backward 165 us (6.7 TB/s); 1021 rows of 131072 f32 logits with 5 alternatives 100 us
-// (5.3 TB/s).
+// forward 116 to 127 us (4.5 TB/s), backward 173 to 180 us (6.2 TB/s); 1021 rows of 131072 f32 logits with 5
+// alternatives 100 us (5.3 TB/s).
 #include <algorithm>
 #include "common.h"
 
