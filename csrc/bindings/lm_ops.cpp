@@ -331,7 +331,7 @@ void embedding_bwd_sorted(torch::Tensor perm, torch::Tensor keys, torch::Tensor 
   // threads of a launch: W / 8 lanes, in groups of up to 64, for each chunk (2 W words of `part`)
   const long long words = tfk_emb_sorted_part(T, (int)W);
   TORCH_CHECK(words / 16 + words / (2 * W) * 64 <= 0x7fffffff, "embedding_bwd_sorted: ", T, " tokens of width ", W, " are too many");
-  TORCH_CHECK((dy.size(1) == 1 || dy.stride(1) == 1) && (T <= 1 || (dy.stride(0) >= W && dy.stride(0) % 8 == 0)),
+  TORCH_CHECK((dy.size(1) == 1 || dy.stride(1) == 1) && (T <= 1 || dy.stride(0) % 8 == 0),  // (0: one row for all tokens)
               "dy rows: unit column stride, row stride a multiple of 8");
   need_aligned(dy, 16, "dy"); need_aligned(dword, 16, "dword");
   need_vec(perm, at::kInt, T, dy, "order"); need_vec(keys, at::kInt, T, dy, "order");

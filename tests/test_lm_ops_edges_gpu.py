@@ -326,3 +326,13 @@ def test_token_order_tiles(T):
     ids = torch.randint(-3, 33003, (T,), generator=torch.Generator().manual_seed(T), dtype=torch.int32)
     a, b = TR.token_order(ids.to(DEV), 33000), TR.token_order(ids, 33000)
     assert torch.equal(a.perm.cpu(), b.perm) and torch.equal(a.keys.cpu(), b.keys)
+
+
+def test_sorted_embedding_of_a_shared_gradient_row():
+    """dy of one row for all tokens (the gradient of a mean, an expanded view)."""
+    ids = zipf(300, 40).to(DEV)
+    row = randn(1, 64, seed=4).to(DEV)
+    o, a, b = TR.token_order(ids, 40), torch.zeros(40, 64, device=DEV), torch.zeros(40, 64, device=DEV)
+    TR.embedding_bwd_sorted(o, row.expand(300, 64), a, scale=0.5)
+    TR.embedding_bwd_sorted(o, row.repeat(300, 1), b, scale=0.5)
+    assert bool(a.any()) and torch.equal(a, b)
