@@ -60,7 +60,7 @@ struct Ty<bf16> {
   }
   static __device__ __forceinline__ x4 tr(const char* p) { return __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS x4*)p); }
   static constexpr bool fits = true;  // has float's exponents
-  static constexpr float p_up = 0.f, raise = 8.f;
+  static constexpr float fwd_up = 0.f, bwd_up = 0.f, raise = 8.f;
 };
 template <>
 struct Ty<f16> {
@@ -73,7 +73,7 @@ struct Ty<f16> {
     return __builtin_bit_cast(x4, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((LDS_AS bf16x4*)p));
   }
   static constexpr bool fits = false;   // 2^-14 .. 2^16
-  static constexpr float p_up = 15.f, raise = 3.f;
+  static constexpr float fwd_up = 15.f, bwd_up = 8.f, raise = 3.f;
 };
 
 struct Shaped {
@@ -289,10 +289,12 @@ __device__ __forceinline__ typename Ty<T>::x8 pack8(const f32x16& a, int half) {
   return r;
 }
 
-// f16 operands. P <= 1 goes into its products times 2^p_up, so it has whole digits down to 2^-29 (unscaled: 2^-14, and a
-// row that gives most of its weight to one key with a small V lost the rest: 16384 keys that share 1%, O off by 0.010
-// of itself, now 0.0003). The forward's P may pass 1 by 2^raise, the log2 units by which a row may outgrow its running
-// maximum before it is rescaled.
+// f16 operands. The forward's P goes into its product times 2^fwd_up and has whole digits down to 2^-29 of the row's
+// maximum (unscaled: 2^-14, and a row that gives most of its weight to one key with a small V lost the rest: 16384 keys
+// that share 1%, O off by 0.010 of itself, now 0.0003); less `raise` in the tiled form, the log2 units by which a row may
+// outgrow its running maximum before it is rescaled. That is f16's largest, so the maximum is taken one or two steps too
+// large (above): the product with the scale rounds, at scores of 1e7 by whole units. The dK/dV pass, whose P comes from
+// the rounded lse and may pass 1 by as much, takes 2^bwd_up (whole digits down to 2^-22).
 // dS = P (dP - delta) (1 - t^2) goes with 1 / keys and with the upstream gradient: unscaled it left f16's range on long
 // rows, for gradients of 1e-3 and smaller (no digits) and of 1e4 (infinite). So a lane's row (dQ) or key (dK) has a
 // power of two `up` for its dS, divided out of the f32 sums at the end: from 2^START,
@@ -415,6 +417,11 @@ struct Score {
 template <typename O>
 __device__ __forceinline__ float slope_of(const Shaped& p, int head) {
   return O::bias && (!O::wide || p.slopes) ? p.slopes[head] * LOG2E : 0.f;
+}
+// a maximum that no score passes by rounding, where P goes up to f16's largest
+template <typename T>
+__device__ __forceinline__ float above(float m) {
+  return Ty<T>::fits ? m : fmaf(fminf(fabsf(m), 1e30f), 0x1p-23f, m);
 }
 // slot r of a 32-row block: row (r & 3) + 8 (r >> 2) (+ 4 h)
 __device__ __forceinline__ constexpr int srow(int r) { return (r & 3) + 8 * (r >> 2); }

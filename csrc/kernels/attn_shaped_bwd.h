@@ -5,7 +5,7 @@
 
 namespace {
 // ------------------------------------------------------------------------------- dQ pass
-// same rows and tiles as the forward; also writes lse in log2 units (shifted, Score; f16: less p_up) and -delta.
+// same rows and tiles as the forward; also writes lse in log2 units (shifted, Score; f16: less bwd_up) and -delta.
 // Precision: delta = sum P dP is taken as dO.O here, off by O's rounding. Beside the roundings of dS and of the
 // gradients this weighs as much as they do where a row's softmax rests on few keys, 1 / n_eff of it else (974 keys
 // under a slope of 1/2 gave 1.7 times the error of a float32 backward, 372 without one 1.48). So where a row of the
@@ -171,7 +171,7 @@ __global__ __launch_bounds__(NW * 64, dq_min_waves(D, O::drop, Ty<T>::fits)) voi
   }
   rest = xor_sum<32>(rest);
   if (valid && h == 0) {  // for the dK/dV pass
-    p.delta[srow_i] = lse2 - Ty<T>::p_up;
+    p.delta[srow_i] = lse2 - Ty<T>::bwd_up;
     p.delta[(long long)p.B * p.H * p.Sq + srow_i] = -(dlt + rest);
   }
   if (valid) {
@@ -299,7 +299,9 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
   for (int db = 0; db < D / 32; ++db)
 #pragma unroll
     for (int e = 0; e < 16; ++e) dk[db][e] = dv[db][e] = 0.f;
-  float up = START * (Ty<T>::fits ? 1.f : 0x1p-15f);  // (f16: P, and with it dS, is 2^15 times itself here)
+  constexpr float P_DOWN = Ty<T>::fits ? 1.f : 0x1p-8f;  // 2^-bwd_up: f16's P, and with it dS, is 2^bwd_up times itself
+  static_assert(Ty<T>::fits || Ty<T>::bwd_up == 8.f, "P_DOWN");
+  float up = START * P_DOWN;
   int g = i0 / max(nt, 1), t = i0 % max(nt, 1);
   if (i0 < i1) landed(0, org + t * KT);
   auto step = [&](auto slot_, int i) {
@@ -412,13 +414,13 @@ __global__ __launch_bounds__(NW * 64, dkv_min_waves(D, O::drop)) void shaped_dkv
     if (i + 1 < i1) step(iconst<1>{}, i + 1);
   }
   if constexpr (!Ty<T>::fits) {
-    const float fk = down(up) * 0x1p-15f;
+    const float fk = down(up) * P_DOWN;
 #pragma unroll
     for (int db = 0; db < D / 32; ++db)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         dk[db][e] *= fk;
-        dv[db][e] *= 0x1p-15f;
+        dv[db][e] *= P_DOWN;
       }
   }
   if (splits > 1) {

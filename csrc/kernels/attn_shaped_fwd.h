@@ -73,7 +73,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
   constexpr bool drop = O::drop;
   const uint32_t hs = drop ? head_seed(p, b * p.H + head) : 0u;
   const int qg = (q >> 2) * p.Sk;
-  constexpr float RAISE = Ty<T>::raise, UP = Ty<T>::fits ? 0.f : Ty<T>::p_up - RAISE;  // P is 2^UP times itself
+  constexpr float RAISE = Ty<T>::raise, UP = Ty<T>::fits ? 0.f : Ty<T>::fwd_up - RAISE;  // P is 2^UP times itself
   float m = -INFINITY, lsum = 0.f;  // lsum: this lane's half of the row
   f32x16 o[D / 32];
 #pragma unroll
@@ -107,6 +107,7 @@ __global__ __launch_bounds__(NW * 64, D == 64 ? 4 : 2) void shaped_fwd_kernel(Sh
       for (int e = 1; e < 16; ++e) mx = fmaxf(mx, s[e]);
       mx = pair_max(mx);
       if (!O::bias) mx = !O::cap ? mx * sc.mult : mx == -INFINITY ? mx : sc.c2l * sc.r(mx);
+      mx = above<T>(mx);
       // the running maximum follows only where a row outgrew it by 2^RAISE: O and the sum are rescaled
       // in few tiles, P stays below 2^RAISE
       if (__any(mx > m + RAISE)) {
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
   const float slope = slope_of<O>(p, head);
   const int pos = q + mk.shift;
   const float fs = O::cap || O::wide ? 1.f : sc.mult, fx = O::bias ? 1.f : fs;  // factors left to the bias, to the exponent
-  constexpr float UP = Ty<T>::p_up;  // P is 2^UP times itself
+  constexpr float UP = Ty<T>::fwd_up;  // P is 2^UP times itself
   float m = -INFINITY, lsum = 0.f;
   f32x16 o[D / 32];
 #pragma unroll
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(FW * 64, 2) void shaped_few_kernel(Shaped p, int sp
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
     mx = pair_max(mx);
-    const float mnew = fmaxf(m, mx * fx), muse = mnew == -INFINITY ? 0.f : mnew, alpha = ex2(m - muse);
+    const float mnew = fmaxf(m, above<T>(mx * fx)), muse = mnew == -INFINITY ? 0.f : mnew, alpha = ex2(m - muse);
     float rs = 0.f;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -413,7 +414,7 @@ __global__ __launch_bounds__(64) void shaped_few_join_kernel(Shaped p, int split
   T* Or = (T*)p.out + b * p.o_bs + q * p.o_rs + head * D;
 #pragma unroll
   for (int u = 0; u < D / 64; ++u) Or[u * 64 + l] = (T)(o[u] * inv);
-  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + (shifted(p) ? p.cap * LOG2E : 0.f) + (__log2f(L) - Ty<T>::p_up)) * LN2 : INFINITY;
+  if (l == 0) p.lse[((long long)b * p.H + head) * p.Sq + q] = L != 0.f ? (M + (shifted(p) ? p.cap * LOG2E : 0.f) + (__log2f(L) - Ty<T>::fwd_up)) * LN2 : INFINITY;
 }
 
 // few rows and no dropout: the split form; shares of a cache so that there are about 4 blocks for each of

@@ -109,6 +109,25 @@ def test_attention_weights_far_below_the_largest(kw, dtype):
     assert float((lse.double().cpu() - r["lse"]).abs().max()) < 2e-5 * 20
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("kw", [dict(Sq=3, Sk=300, causal=True, q_start=[297], fused=False), dict(Sq=1, Sk=1500, H=4, D=128, fused=False),
+                                dict(Sq=150, causal=True, prefix_len=[0]), dict(Sq=140, H=1, D=128), dict(Sq=100, slopes=1.0)],
+                         ids=["few", "few_wide", "tiles", "tiles_wide", "tiles_bias"])
+def test_attention_scores_past_float32_integers(kw, dtype):
+    """Scores of 1e7 to 1e8, where a float32 step is 1 to 8: a row takes its best key, nothing overflows."""
+    c = Case(B=1, dtype=dtype, scale=4000.0, seed=11, **kw)
+    c.v = c.v / 4000
+    c.check(grads=False)
+    c = Case(B=1, dtype=dtype, scale=1500.0, seed=11, **kw)
+    c.v = c.v / 1500
+    sp = c.spec()
+    out, lse = TR.attention_fwd(sp)
+    d = [torch.empty_like(t[0]) for t in (sp.q, sp.k, sp.v)]
+    TR.attention_bwd(sp, out, c.dout.reshape(out.shape).to(DEV), lse, *((x, t[1]) for x, t in zip(d, (sp.q, sp.k, sp.v))))
+    n = [c.H * c.D, c.Hk * c.D, c.Hk * c.D]
+    assert all(torch.isfinite(x[:, t[1]:t[1] + w]).all() for x, t, w in zip(d, (sp.q, sp.k, sp.v), n))
+
+
 # ------------------------------------------------------------------------------------- any score cap
 
 @pytest.mark.parametrize("cap", [1.2e-38, 1e-30, 1e-3, 128.0, 512.0, 513.0, 1e4, 1e6, 1e8, 1e30, 2e38])
