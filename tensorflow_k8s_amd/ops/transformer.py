@@ -329,7 +329,7 @@ class AttnSpec:
     Shaped scores (any of the keyword arguments below; bf16 or f16, head_dim 64 or 128):
       score(i, j) = softcap tanh(scale q_i.k_j / softcap) - slopes[h] |p_i - j|
     kv_heads    key/value heads; query heads h G .. h G + G - 1 (G = H / kv_heads) share key head h
-    softcap     > 0: tanh cap of the scaled scores
+    softcap     > 0: tanh cap of the scaled scores (any size; above 512 by a slower form)
     slopes      f32 [H]: bias by distance (constants: no gradient)
     q_start     int32 [B]: query i of batch b stands at key position p_i = i + q_start[b] (default 0)
     prefix_len  int32 [B], with causal: keys below it are seen by every query, else key j by p_i >= j
@@ -340,7 +340,7 @@ class AttnSpec:
     padding, other documents) may hold anything; a non-finite value in a key that some queries see can
     reach the others of the same tile. Buffers may be 2-D [B*S, width] or 3-D [B, S', width]
     with S' >= S (a cache with room; it takes the shaped kernels by itself, a contiguous one of S tokens does not),
-    rows any multiple of 8 elements apart."""
+    rows any multiple of 8 elements apart (below 2^23)."""
 
     def __init__(self, B, H, Sq, Sk, q, k, v, kv_len=None, causal=False, p_drop=0.0, seed=0, scale=None, *,
                  kv_heads=None, head_dim=HEAD_DIM, softcap=0.0, slopes=None, docs=None, prefix_len=None,
