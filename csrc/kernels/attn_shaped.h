@@ -97,9 +97,9 @@ struct Shaped {
 // Caps up to here take the shifted form of a score (Score), larger ones the wide form. The shift puts the float32 step of
 // cap on every score: f16, S 600, relative error of O (0.00020: rounded once) and absolute one of lse are 0.000256 and 1e-5 at
 // a cap of 128, 0.000255 and 4e-5 at 512, 0.000258 and 6e-5 at 1024, 0.00049 and 7e-4 at 1e4, 0.0037 and 8e-3 at 1e5; the
-// wide form's 0.000254 and 1e-6 at any cap, for up to half more time (B1 H16/4 S8192 D128 bf16:
-// forward 351 -> 540 us, backward 1021 -> 1323).
-constexpr float CAP_SHIFT = 512.f;
+// wide form's 0.000254 and 1e-6 at any cap, for up to half more time (B1 H16/4 S8192 D128 bf16: forward 351 -> 540 us,
+// backward 1021 -> 1323). 128 keeps an lse near 0 to 2e-5: half a step of the shift and one of its reciprocal.
+constexpr float CAP_SHIFT = 128.f;
 __host__ __device__ __forceinline__ bool shifted(const Shaped& p) { return p.cap > 0.f && p.cap <= CAP_SHIFT; }
 
 // the score rules of a call, compiled in: as runtime branches their joins cost the dK/dV pass 40 registers

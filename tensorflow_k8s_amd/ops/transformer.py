@@ -329,7 +329,7 @@ class AttnSpec:
     Shaped scores (any of the keyword arguments below; bf16 or f16, head_dim 64 or 128):
       score(i, j) = softcap tanh(scale q_i.k_j / softcap) - slopes[h] |p_i - j|
     kv_heads    key/value heads; query heads h G .. h G + G - 1 (G = H / kv_heads) share key head h
-    softcap     > 0: tanh cap of the scaled scores (any size; above 512 by a slower form)
+    softcap     > 0: tanh cap of the scaled scores (any size; above 128 by a slower form)
     slopes      f32 [H]: bias by distance (constants: no gradient)
     q_start     int32 [B]: query i of batch b stands at key position p_i = i + q_start[b] (default 0)
     prefix_len  int32 [B], with causal: keys below it are seen by every query, else key j by p_i >= j

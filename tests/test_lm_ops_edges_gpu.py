@@ -130,7 +130,7 @@ def test_attention_scores_past_float32_integers(kw, dtype):
 
 # ------------------------------------------------------------------------------------- any score cap
 
-@pytest.mark.parametrize("cap", [1.2e-38, 1e-30, 1e-3, 128.0, 512.0, 513.0, 1e4, 1e6, 1e8, 1e30, 2e38])
+@pytest.mark.parametrize("cap", [1.2e-38, 1e-30, 1e-3, 128.0, 129.0, 512.0, 513.0, 1e4, 1e6, 1e8, 1e30, 2e38])
 @pytest.mark.parametrize("kw", [
     dict(B=1, H=2, Hk=1, Sq=150, causal=True),
     dict(B=1, H=2, Hk=1, D=128, Sq=140, causal=True, dtype=HF, slopes=True, doc_ids=docs(1, 140, [60, 29], pad=7)),
@@ -142,11 +142,20 @@ def test_attention_any_cap(kw, cap):
     Case(cap=cap, **kw).check()
 
 
-@pytest.mark.parametrize("cap", [1e-30, 512.0, 513.0, 1e6, 1e30])
+@pytest.mark.parametrize("cap", [1e-30, 128.0, 129.0, 512.0, 513.0, 1e6, 1e30])
 @pytest.mark.parametrize("Sk", [300, 1500])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_attention_any_cap_few_rows(dtype, Sk, cap):
     Case(B=2, H=4, Hk=2, D=128, Sq=2, Sk=Sk, causal=True, kv_len=[Sk, 9], q_start=[Sk - 2, 7], cap=cap, dtype=dtype, fused=False).check(grads=False)
+
+
+@pytest.mark.parametrize("cap", [30.0, 128.0, 129.0, 512.0, 1e4])
+@pytest.mark.parametrize("Sq", [1, 40])
+def test_attention_any_cap_lse_near_0(cap, Sq):
+    """One key with a score near 0: lse is that score, within 2e-5 (the score's own digits are far below)."""
+    for D in (64, 128):
+        for seed in range(40):
+            Case(B=1, H=2, Sq=Sq, Sk=1, D=D, cap=cap, fused=False, seed=4 * seed, scale=0.3).check(grads=False)
 
 
 # ------------------------------------------------------------------------------------- strides of lone tokens
